@@ -20,29 +20,29 @@ TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 def listed():
     return [
         # a decoder with four heads over the paper-size Listener: 32 utterances of 800 frames (T' = 100), 128 characters
-        dict(name="attend train, 32 x 128 over 100", op="train", type="fp32", B=32, U=128, T=100, H=4, Hkv=4, D=128),
+        dict(name="attend train 32x128 over 100", op="train", type="fp32", B=32, U=128, T=100, H=4, Hkv=4, D=128),
         # the long-utterance batch (3000 frames, T' = 375) in 16 bits
-        dict(name="attend train, 8 x 128 over 375", op="train", type="bf16", B=8, U=128, T=375, H=8, Hkv=8, D=64),
+        dict(name="attend train 8x128 over 375", op="train", type="bf16", B=8, U=128, T=375, H=8, Hkv=8, D=64),
         # a large training batch with four query heads to a key head
-        dict(name="attend train, 16 x 512 over 1500", op="train", type="bf16", B=16, U=512, T=1500, H=16, Hkv=4, D=64),
+        dict(name="attend train 16x512 over 1500", op="train", type="bf16", B=16, U=512, T=1500, H=16, Hkv=4, D=64),
         # scoring given transcripts against long recordings, no gradient; ragged sizes
-        dict(name="attend, 4 x 333 over 2999", op="attend", type="fp32", B=4, U=333, T=2999, H=8, Hkv=8, D=64),
+        dict(name="attend 4x333 over 2999", op="attend", type="fp32", B=4, U=333, T=2999, H=8, Hkv=8, D=64),
         # one decode step of a validation batch: latency
-        dict(name="attend one token, 32 over 375", op="attend", type="bf16", B=32, U=1, T=375, H=8, Hkv=8, D=64),
+        dict(name="one token 32 over 375", op="attend", type="bf16", B=32, U=1, T=375, H=8, Hkv=8, D=64),
         # one decode step over hours of sound: the features of 16 streams are read once
-        dict(name="attend one token, 16 over 30000", op="attend", type="fp16", B=16, U=1, T=30000, H=16, Hkv=4, D=128),
+        dict(name="one token 16 over 30000", op="attend", type="fp16", B=16, U=1, T=30000, H=16, Hkv=4, D=128),
         # a character model taught by a larger one: the Speller's own vocabulary
-        dict(name="distill, characters", op="distill", type="fp32", B=32, U=128, V=30, K=8),
+        dict(name="distill characters", op="distill", type="fp32", B=32, U=128, V=30, K=8),
         # subword vocabulary, odd sizes
-        dict(name="distill, 5003 subwords", op="distill", type="fp32", B=16, U=201, V=5003, K=32),
+        dict(name="distill 5003 subwords", op="distill", type="fp32", B=16, U=201, V=5003, K=32),
         # a large vocabulary in 16 bits: logits read and their gradient written once
-        dict(name="distill, 128000 tokens", op="distill", type="bf16", B=8, U=512, V=128000, K=64),
+        dict(name="distill 128000 tokens", op="distill", type="bf16", B=8, U=512, V=128000, K=64),
         # one step of the Speller's batch
-        dict(name="sample, characters", op="sample", type="fp32", B=32, V=30, top_k=0, top_p=0.9, min_p=0.02, temperature=0.8, per_row=False),
+        dict(name="sample characters", op="sample", type="fp32", B=32, V=30, top_k=0, top_p=0.9, min_p=0.02, temperature=0.8, per_row=False),
         # a serving batch with all filters, each row its own temperature
-        dict(name="sample, 64 of 32000", op="sample", type="bf16", B=64, V=32000, top_k=50, top_p=0.9, min_p=0.01, temperature=0.5, per_row=True),
+        dict(name="sample 64 of 32000", op="sample", type="bf16", B=64, V=32000, top_k=50, top_p=0.9, min_p=0.01, temperature=0.5, per_row=True),
         # one row of a large vocabulary, no limit on the candidates but their mass
-        dict(name="sample, 1 of 128000", op="sample", type="fp32", B=1, V=128000, top_k=0, top_p=0.95, min_p=0.0, temperature=1.0, per_row=False),
+        dict(name="sample 1 of 128000", op="sample", type="fp32", B=1, V=128000, top_k=0, top_p=0.95, min_p=0.0, temperature=1.0, per_row=False),
     ]
 
 
