@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define LAS_ABI_VERSION 10
+#define LAS_ABI_VERSION 11
 #define LAS_MAX_SPELLER_LAYERS 4
 
 /* flags */
@@ -247,6 +247,31 @@ int las_speller_bwd(const las_speller_desc* d, const float* feat, const float* k
                     const float* logp, const float* att, const float* dlogp, int U, int feedback_mode0,
                     const float* reserve, float* workspace, const las_speller_grads* g, uint32_t* err_word, int flags,
                     void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Attention of decoder states over an encoder's states of another length.  Beside las_attention_*, which attends one decoder state per
+ * utterance with the reference's MLP keys (model/las_model.py:275-318): here U states per utterance, H query heads that share Hkv key /
+ * value heads (H a multiple of Hkv; query head h reads head h / (H / Hkv)), and utterances of different lengths.
+ *   s[i][j] = scale q_i . k_j over the first key_lengths[b] of T frames,  out_i = sum_j softmax_j(s)[i][j] v_j
+ *   An utterance without valid frames gives out = 0 and zero gradients.  What the frames behind key_lengths[b] hold is never read (dk / dv are
+ *   written there, as zeros).  key_lengths: int32 (B) on the device, values outside [0, T] count as the nearer end; NULL: every frame is valid.
+ *   q (B,U,H,D), k / v (B,T,Hkv,D) of one type (dtype 0 fp32, 1 bf16, 2 fp16), any strides (in elements) with rows of D contiguous; row
+ *   starts 16-byte aligned; D <= 128, a multiple of 16 bytes.  out / dout / dq (B,U,H,D) and dk / dv (B,T,Hkv,D) contiguous.
+ *   lse (B,U,H) fp32: log2 of the sum of exp(s), or -inf; NULL in a forward that no backward follows.  Scores, softmax and sums are fp32.
+ *   workspace: las_cross_attention_workspace_floats() floats (0: may be NULL), private to the call until its kernels have run.
+ *   No atomics: results are the same from run to run.  Any stream, capturable.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct las_cross_attention_desc {
+    int B, U, T, H, Hkv, D, dtype;
+    float scale;
+    int64_t q_b, q_u, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
+} las_cross_attention_desc;
+size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d, int backward);
+int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                            void* out, float* lse, float* workspace, void* stream);
+int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* workspace,
+                            void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Caller-side contract on device (the code that CALLS the hot path, reference solver/solver.py).

@@ -4,6 +4,7 @@ reference's ``Listener`` / ``Speller`` / ``LAS`` nn.Module surface.  All arithme
 HIP kernels (``csrc/``) reached through a C ABI (``include/las_hip.h``); PyTorch only owns memory,
 streams, autograd bookkeeping and ``torch.distributed``."""
 from ._cabi import check_device_errors  # noqa: F401
+from .model.cross_attention import cross_attention  # noqa: F401
 from .model.las_model import LAS, Attention, Listener, Speller, pBLSTMLayer  # noqa: F401
 
-__all__ = ["LAS", "Listener", "Speller", "Attention", "pBLSTMLayer", "check_device_errors"]
+__all__ = ["LAS", "Listener", "Speller", "Attention", "pBLSTMLayer", "cross_attention", "check_device_errors"]

@@ -43,6 +43,11 @@ class SpellerGrads(C.Structure):
                 ("dw_dr", _f), ("db_dr", _f), ("dfeat", _f)]
 
 
+class CrossAttentionDesc(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("B", "U", "T", "H", "Hkv", "D", "dtype")] + [("scale", C.c_float)]
+                + [(n, C.c_int64) for n in ("q_b", "q_u", "q_h", "k_b", "k_t", "k_h", "v_b", "v_t", "v_h")])
+
+
 # name -> (restype, argtypes); every symbol include/las_hip.h declares
 PROTOTYPES = {
     "las_abi_version": (C.c_int, []),
@@ -83,6 +88,9 @@ PROTOTYPES = {
     "las_speller_bwd_workspace_floats": (C.c_size_t, [C.POINTER(SpellerDesc), C.c_int]),
     "las_speller_bwd": (C.c_int, [C.POINTER(SpellerDesc), _f, _f, _f, _f, _f, C.c_int, C.c_int, _f, _f,
                                   C.POINTER(SpellerGrads), _f, C.c_int, _f]),
+    "las_cross_attention_workspace_floats": (C.c_size_t, [C.POINTER(CrossAttentionDesc), C.c_int]),
+    "las_cross_attention_fwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 8),
+    "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 12),
     "las_ls_loss": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _f, _f, C.c_int64,
                               C.c_int64, _f, _f]),
     "las_letter_error_rate": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, _f, _f, _f]),
@@ -174,6 +182,16 @@ def ptr_strided(t):
 
 def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
+
+
+def call_on(device, fn, *args):
+    """``check(fn(*args, stream))`` with ``device`` current and its current stream: a launch goes to the device that is current, whatever its
+    operands live on."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
 
 
 _err_words = {}

@@ -1,0 +1,652 @@
+// Attention of decoder states over an encoder's states of another length: forward, one-token form, backward.
+//
+//   s[i][j] = scale q_i . k_j  (j < len_b),  p = softmax_j s,  o_i = sum_j p[i][j] v_j ;  len_b = 0: o = 0 and every gradient 0.
+//   D_i = do_i . o_i,  ds = p (do_i . v_j - D_i),  dq_i = scale sum_j ds k_j,  dk_j = scale sum_i ds q_i,  dv_j = sum_i p do_i.
+//
+// Heads: H query heads share Hkv key / value heads in groups of G = H / Hkv.  The rows of one (utterance, key head) are its G U query
+// rows, numbered u G + g, so a tile of rows may span heads: a decode step of grouped heads is one tile, dk / dv of a shared head are
+// summed over its group inside one workgroup — no atomics anywhere, every sum has a fixed order.
+//
+// One pass over the keys with the running maximum and sum of the softmax (fp32).  The score tile is formed TRANSPOSED (keys x rows:
+// keys along the accumulator registers, one row per lane), so a row's maximum and sum are register reductions plus one exchange
+// between the wave's halves, the rescale factor is one value per lane, and the probabilities leave the matrix instruction in just
+// the shape that the second product wants as its right operand once the keys are taken in the order in which they lie in registers
+// (a contraction may take its index in any order, if both operands do).  The left operand of that product (V^T, and K^T / Q^T / dO^T in
+// the backward) is read from the row-major tile by the transposing LDS load for 16-bit types, by plain dword loads for fp32.
+#include "las_common.h"
+#include "las_kernels.h"
+#include <math.h>
+
+namespace las {
+namespace {
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using f32x8 = __attribute__((ext_vector_type(8))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+
+constexpr int CA_THREADS = 256;
+
+// ---- the matrix instruction by type: one 16-byte chunk per lane of either operand -------------------------------------------
+// 16-bit: one 32x32x16 (lane half h holds contraction indices 8 h .. 8 h + 7 of 16).  fp32: four 32x32x2 (index 4 h + j of 8 in step j).
+template <class T> struct Mma;
+template <> struct Mma<__bf16> {
+    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<_Float16> {
+    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma<float> {
+    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// geometry of one type: EL elements per 16-byte chunk, a chunk of both lane halves covers CH contraction indices
+template <class T, int DP> struct Geo {
+    static constexpr int EL = 16 / (int)sizeof(T), CH = 2 * EL, NCH = DP / CH, LD = DP + EL, CPR = DP / EL, NDT = DP / 32;
+    static constexpr int PCH = 32 / CH;        // chunks of a 32-row contraction
+};
+
+// chunk c of the 32x32 accumulator tile as the right operand of the next product: accumulator register r of lane half h is row
+// 8 (r / 4) + 4 h + r % 4, so a 16-bit chunk (registers 8 c .. 8 c + 7) holds rows 16 c + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} and a
+// fp32 chunk (registers 4 c .. 4 c + 3) rows 8 c + 4 h .. + 3.  ld_t below reads the left operand in the same order.
+// Rounding P and dS to the inputs' 16 bits costs half a step (2^-9 bf16, 2^-12 fp16) per term of sums that stay in fp32.
+template <class T> static __device__ __forceinline__ u32x4 pack(const f32x16& x, int c) {
+    if constexpr (sizeof(T) == 4) {
+        f32x4 y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+        return __builtin_bit_cast(u32x4, y);
+    } else {
+        using V8 = __attribute__((ext_vector_type(8))) T;
+        f32x8 y = {x[8 * c], x[8 * c + 1], x[8 * c + 2], x[8 * c + 3], x[8 * c + 4], x[8 * c + 5], x[8 * c + 6], x[8 * c + 7]};
+        return __builtin_bit_cast(u32x4, __builtin_convertvector(y, V8));
+    }
+}
+
+// fp16 keeps its full precision only above 2^-14: probabilities are formed 2^14 times too large there (at most 2^14 of 65504; a power of two in
+// the exponential's argument costs nothing) and the sums divided by it, so that a probability is good to half a step down to 2^-28.
+template <class T> constexpr float P_SHIFT = 0.f;
+template <> constexpr float P_SHIFT<_Float16> = 14.f;
+
+// left operand, row-major: chunk c of row `row` of an LDS tile
+template <class T, int DP> static __device__ __forceinline__ u32x4 ld_row(const T* s, int row, int c, int h) {
+    using G = Geo<T, DP>;
+    return *(const u32x4*)(s + row * G::LD + c * G::CH + h * G::EL);
+}
+
+// left operand, transposed: column d0 + lane % 32 of the tile at the contraction rows of chunk c (order: see pack), counted from row0
+template <class T, int DP> static __device__ __forceinline__ u32x4 ld_t(const T* s, int row0, int c, int d0, int lane) {
+    using G = Geo<T, DP>;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+        const float* p = (const float*)s + (row0 + 8 * c + 4 * h) * G::LD + d0 + (lane & 31);
+        f32x4 y = {p[0], p[G::LD], p[2 * G::LD], p[3 * G::LD]};
+        return __builtin_bit_cast(u32x4, y);
+    } else {
+        // ds_read_b64_tr_b16: the 16 lanes of a group name the 16 eight-byte pieces of a 4 (rows) x 16 (columns) block; lane i receives column i
+        const int i = lane & 15;
+        const T* p = s + (row0 + 16 * c + 4 * h + (i >> 2)) * G::LD + d0 + (lane & 16) + (i & 3) * 4;
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * G::LD));
+        struct { s16x4 a, b; } both = {lo, hi};
+        return __builtin_bit_cast(u32x4, both);
+    }
+}
+
+// ---- tiles of rows between global memory, registers and LDS -----------------------------------------------------------------
+// Rows of any stride (multiples of 16 bytes); what lies outside [0, nrows) x [0, D) reads as zero, so that whatever a masked place
+// holds (infinities, NaN) never meets a product.
+template <class T, int DP, int ROWS> struct RowTile {
+    using G = Geo<T, DP>;
+    static constexpr int N = (ROWS * G::CPR + CA_THREADS - 1) / CA_THREADS;
+    u32x4 r[N];
+    __device__ __forceinline__ void load(const T* base, long stride, int nrows, int D, int tid) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
+            r[v] = u32x4{0, 0, 0, 0};
+            if (row < nrows && row < ROWS && ch * G::EL < D) r[v] = *(const u32x4*)(base + row * stride + ch * G::EL);
+        }
+    }
+    // rows of the (u, g) numbering: row n = u G + g lies at u su + g sg
+    __device__ __forceinline__ void load_rows(const T* base, long su, long sg, int row0, int nrows, int share, int D, int tid) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
+            r[v] = u32x4{0, 0, 0, 0};
+            if (row0 + row < nrows && row < ROWS && ch * G::EL < D) {
+                const int u = share == 1 ? row0 + row : (row0 + row) / share, g = row0 + row - u * share;
+                r[v] = *(const u32x4*)(base + u * su + g * sg + ch * G::EL);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* s, int tid) const {
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
+            if (ROWS * G::CPR % CA_THREADS == 0 || row < ROWS) *(u32x4*)(s + row * G::LD + ch * G::EL) = r[v];
+        }
+    }
+};
+
+static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// Workgroups of one (utterance, key head) read the same keys: give each XCD (blockIdx % 8 on this device) a contiguous run of work so that
+// they share its L2.  A permutation of [0, n) for any n: correct whatever the placement.
+static __device__ __forceinline__ int xcd_order(int b, int n) {
+    const int per = n >> 3, rem = n & 7, x = b & 7, i = b >> 3;
+    return x * per + min(x, rem) + i;
+}
+
+static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
+    return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------
+// Four waves: NWQ of them side by side over rows (32 each), NWK over keys (KT tiles of 32 of every key tile each).
+template <class T, int DP, int NWQ, int NWK, int KT>
+__global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArgs a) {
+    using G = Geo<T, DP>;
+    constexpr int BK = 32 * KT * NWK;
+    constexpr int RED = NWK > 1 ? 4 * (DP + 2) * 32 * 4 : 0;                    // bytes of the joining of waves
+    constexpr int TILE = 2 * BK * G::LD * (int)sizeof(T);
+    __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
+    T* sK = (T*)smem;
+    T* sV = sK + BK * G::LD;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
+    const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
+    const int w = xcd_order(blockIdx.x, gridDim.x);
+    const int tile = w % ntiles, split = (w / ntiles) % a.nsplit, bh = w / (ntiles * a.nsplit), b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int len = length_of(a, b);
+    const int per = ((len + a.nsplit - 1) / a.nsplit + 31) & ~31;
+    const int begin = min(len, split * per), end = min(len, begin + per);
+    const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
+    const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
+    const T* v = (const T*)a.v + b * a.v_b + kvh * a.v_h;
+
+    const int row = tile * 32 * NWQ + wq * 32 + (lane & 31), u = row / share, g = row - u * share;
+    const bool live = row < R;
+    u32x4 qf[G::NCH];
+#pragma unroll
+    for (int c = 0; c < G::NCH; ++c) {
+        qf[c] = u32x4{0, 0, 0, 0};
+        const int d = c * G::CH + h * G::EL;
+        if (live && d < a.D) qf[c] = *(const u32x4*)(q + u * a.q_u + g * a.q_h + d);
+    }
+    f32x16 acc[G::NDT];
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
+    float m = -INFINITY, l = 0.f;
+
+    RowTile<T, DP, BK> tk, tv;
+    if (begin < end) {
+        tk.load(k + (long)begin * a.k_t, a.k_t, end - begin, a.D, tid);
+        tv.load(v + (long)begin * a.v_t, a.v_t, end - begin, a.D, tid);
+    }
+    for (int k0 = begin; k0 < end; k0 += BK) {
+        __syncthreads();
+        tk.store(sK, tid);
+        tv.store(sV, tid);
+        __syncthreads();
+        if (k0 + BK < end) {
+            tk.load(k + (long)(k0 + BK) * a.k_t, a.k_t, end - k0 - BK, a.D, tid);
+            tv.load(v + (long)(k0 + BK) * a.v_t, a.v_t, end - k0 - BK, a.D, tid);
+        }
+        if (k0 + wk * KT * 32 >= end) continue;      // (wave-uniform; the barriers above are met by every wave again)
+        f32x16 s[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            s[t] = f32x16{0};
+#pragma unroll
+            for (int c = 0; c < G::NCH; ++c) s[t] = Mma<T>::run(s[t], ld_row<T, DP>(sK, (wk * KT + t) * 32 + (lane & 31), c, h), qf[c]);
+        }
+        if (k0 + (wk * KT + KT) * 32 > end) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (k0 + (wk * KT + t) * 32 + 8 * (r >> 2) + 4 * h + (r & 3) >= end) s[t][r] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+        mx = fmaxf(m, fmaxf(mx, other_half(mx)));
+        if (__any(mx > m)) {
+            const float alpha = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mx) * a.c);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+            m = mx;
+        }
+        const float mc = (m == -INFINITY ? 0.f : m * a.c) - P_SHIFT<T>;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.c, -mc));
+                l += s[t][r];
+            }
+#pragma unroll
+            for (int c = 0; c < G::PCH; ++c) {
+                const u32x4 p = pack<T>(s[t], c);
+#pragma unroll
+                for (int i = 0; i < G::NDT; ++i) acc[i] = Mma<T>::run(acc[i], ld_t<T, DP>(sV, (wk * KT + t) * 32, c, i * 32, lane), p);
+            }
+        }
+    }
+    l += other_half(l);
+    if constexpr (NWK > 1) {       // join the waves of one row tile, in their order
+        float* red = (float*)smem;
+        float* mine = red + wave * (DP + 2) * 32;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mine[(i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)] = acc[i][r];
+        if (h == 0) { mine[DP * 32 + lane] = m; mine[(DP + 1) * 32 + lane] = l; }
+        __syncthreads();
+        if (wk != 0) return;
+        const float* first = red + wq * NWK * (DP + 2) * 32;
+        float mj = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < NWK; ++x) mj = fmaxf(mj, first[x * (DP + 2) * 32 + DP * 32 + (lane & 31)]);
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
+#pragma unroll
+        for (int x = 0; x < NWK; ++x) {
+            const float* from = first + x * (DP + 2) * 32;
+            const float mm = from[DP * 32 + (lane & 31)];
+            const float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mm - mj) * a.c);
+            l += f * from[(DP + 1) * 32 + (lane & 31)];
+#pragma unroll
+            for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    acc[i][r] = fmaf(f, from[(i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)], acc[i][r]);
+        }
+        m = mj;
+    }
+    if (!live) return;
+    const long out_row = ((long)b * a.U + u) * a.H + kvh * share + g;
+    if (a.nsplit > 1) {
+        const long at = (long)split * a.B * a.U * a.H + out_row;
+        float* part = a.part + at * a.D;
+#pragma unroll
+        for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = i * 32 + 8 * x + 4 * h;
+                if (d < a.D) *(f32x4*)(part + d) = f32x4{acc[i][4 * x], acc[i][4 * x + 1], acc[i][4 * x + 2], acc[i][4 * x + 3]};
+            }
+        if (h == 0) {
+            float* ml = a.part + (long)a.nsplit * a.B * a.U * a.H * a.D + at * 2;
+            ml[0] = m; ml[1] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);        // (no key at all: zeros; a NaN stays one)
+    T* o = (T*)a.o + out_row * a.D;
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = i * 32 + 8 * x + 4 * h;
+            using V4 = __attribute__((ext_vector_type(4))) T;
+            const f32x4 y = {acc[i][4 * x] * inv, acc[i][4 * x + 1] * inv, acc[i][4 * x + 2] * inv, acc[i][4 * x + 3] * inv};
+            if (d < a.D) *(V4*)(o + d) = __builtin_convertvector(y, V4);
+        }
+    if (a.lse && h == 0) a.lse[out_row] = l > 0.f ? fmaf(m, a.c, log2f(l) - P_SHIFT<T>) : (l == 0.f ? -INFINITY : l);
+}
+
+// joins the key ranges of a split forward: four values of one row per thread
+template <class T>
+__global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnArgs a) {
+    const long n = (long)a.B * a.U * a.H, per = a.D / 4, i = (long)blockIdx.x * CA_THREADS + threadIdx.x;
+    if (i >= n * per) return;
+    const long row = i / per;
+    const int d = (int)(i - row * per) * 4;
+    const float* ml = a.part + (long)a.nsplit * n * a.D;
+    float mj = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) mj = fmaxf(mj, ml[(s * n + row) * 2]);
+    f32x4 acc = {0, 0, 0, 0};
+    float l = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float m = ml[(s * n + row) * 2], ls = ml[(s * n + row) * 2 + 1];
+        if (ls == 0.f) continue;                       // (an empty range)
+        const float f = __builtin_amdgcn_exp2f((m - mj) * a.c);
+        const f32x4 x = *(const f32x4*)(a.part + (s * n + row) * a.D + d);
+        l += f * ls;
+        acc += f * x;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    using V4 = __attribute__((ext_vector_type(4))) T;
+    acc *= inv;
+    *(V4*)((T*)a.o + row * a.D + d) = __builtin_convertvector(acc, V4);
+    if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT<T>) : (l == 0.f ? -INFINITY : l);
+}
+
+// ---- backward: dq (and D_i) -------------------------------------------------------------------------------------------------
+// The forward's shape: one row per lane; q and do stay in registers, every key tile is read once per row tile.
+template <class T, int DP, int NWQ, int NWK, int KT>
+__global__ __launch_bounds__(CA_THREADS) void cross_attn_dq_kernel(CrossAttnArgs a) {
+    using G = Geo<T, DP>;
+    constexpr int BK = 32 * KT * NWK;
+    constexpr int RED = NWK > 1 ? 4 * DP * 32 * 4 : 0;
+    constexpr int TILE = 2 * BK * G::LD * (int)sizeof(T);
+    __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
+    T* sK = (T*)smem;
+    T* sV = sK + BK * G::LD;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
+    const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
+    const int w = xcd_order(blockIdx.x, gridDim.x);
+    const int tile = w % ntiles, bh = w / ntiles, b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int end = length_of(a, b);
+    const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
+    const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
+    const T* v = (const T*)a.v + b * a.v_b + kvh * a.v_h;
+    const int row = tile * 32 * NWQ + wq * 32 + (lane & 31), u = row / share, g = row - u * share;
+    const bool live = row < R;
+    const long out_row = ((long)b * a.U + u) * a.H + kvh * share + g;
+
+    RowTile<T, DP, BK> tk, tv;
+    if (end > 0) {
+        tk.load(k, a.k_t, end, a.D, tid);
+        tv.load(v, a.v_t, end, a.D, tid);
+    }
+    u32x4 qf[G::NCH], dof[G::NCH];
+    float delta = 0.f;
+#pragma unroll
+    for (int c = 0; c < G::NCH; ++c) {
+        qf[c] = dof[c] = u32x4{0, 0, 0, 0};
+        const int d = c * G::CH + h * G::EL;
+        if (live && d < a.D) {
+            using VE = __attribute__((ext_vector_type(G::EL))) T;
+            qf[c] = *(const u32x4*)(q + u * a.q_u + g * a.q_h + d);
+            dof[c] = *(const u32x4*)((const T*)a.dout + out_row * a.D + d);
+            const VE x = *(const VE*)((const T*)a.o + out_row * a.D + d), y = __builtin_bit_cast(VE, dof[c]);
+#pragma unroll
+            for (int e = 0; e < G::EL; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+        }
+    }
+    delta += other_half(delta);
+    if (live && wk == 0 && h == 0) a.delta[out_row] = delta;
+    const float lse = live ? a.lse[out_row] : INFINITY;
+    f32x16 acc[G::NDT];
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
+
+    for (int k0 = 0; k0 < end; k0 += BK) {
+        __syncthreads();
+        tk.store(sK, tid);
+        tv.store(sV, tid);
+        __syncthreads();
+        if (k0 + BK < end) {
+            tk.load(k + (long)(k0 + BK) * a.k_t, a.k_t, end - k0 - BK, a.D, tid);
+            tv.load(v + (long)(k0 + BK) * a.v_t, a.v_t, end - k0 - BK, a.D, tid);
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            const int r0 = (wk * KT + t) * 32;
+            if (k0 + r0 >= end) continue;
+            f32x16 s = f32x16{0}, dp = f32x16{0};
+#pragma unroll
+            for (int c = 0; c < G::NCH; ++c) {
+                s = Mma<T>::run(s, ld_row<T, DP>(sK, r0 + (lane & 31), c, h), qf[c]);
+                dp = Mma<T>::run(dp, ld_row<T, DP>(sV, r0 + (lane & 31), c, h), dof[c]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
+                s[r] = k0 + r0 + 8 * (r >> 2) + 4 * h + (r & 3) < end ? p * (dp[r] - delta) : 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < G::PCH; ++c) {
+                const u32x4 ds = pack<T>(s, c);
+#pragma unroll
+                for (int i = 0; i < G::NDT; ++i) acc[i] = Mma<T>::run(acc[i], ld_t<T, DP>(sK, r0, c, i * 32, lane), ds);
+            }
+        }
+    }
+    if constexpr (NWK > 1) {
+        float* red = (float*)smem;
+        __syncthreads();
+        if (wk != 0) {
+#pragma unroll
+            for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) red[(wave * DP + i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)] = acc[i][r];
+        }
+        __syncthreads();
+        if (wk != 0) return;
+#pragma unroll
+        for (int x = 1; x < NWK; ++x)
+#pragma unroll
+            for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][r] += red[((wave + x) * DP + i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)];
+    }
+    if (!live) return;
+    T* o = (T*)a.dq + out_row * a.D;
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = i * 32 + 8 * x + 4 * h;
+            using V4 = __attribute__((ext_vector_type(4))) T;
+            const f32x4 y = {acc[i][4 * x] * a.scale, acc[i][4 * x + 1] * a.scale, acc[i][4 * x + 2] * a.scale, acc[i][4 * x + 3] * a.scale};
+            if (d < a.D) *(V4*)(o + d) = __builtin_convertvector(y, V4);
+        }
+}
+
+// ---- backward: dk, dv -------------------------------------------------------------------------------------------------------
+// One key per lane (k and v in registers), row tiles of q and do through LDS; NWK waves side by side over keys, NWR over rows.
+template <class T, int DP, int NWK, int NWR, int RT>
+__global__ __launch_bounds__(CA_THREADS) void cross_attn_dkv_kernel(CrossAttnArgs a) {
+    using G = Geo<T, DP>;
+    constexpr int BR = 32 * RT * NWR;
+    constexpr float P_BACK = P_SHIFT<T> == 0.f ? 1.f : 1.f / 16384.f;
+    constexpr int RED = NWR > 1 ? 4 * DP * 32 * 4 : 0;
+    constexpr int TILE = 2 * BR * G::LD * (int)sizeof(T) + 2 * BR * 4;
+    __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
+    T* sQ = (T*)smem;
+    T* sO = sQ + BR * G::LD;
+    float* sL = (float*)(sO + BR * G::LD);
+    float* sD = sL + BR;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
+    const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
+    const int w = xcd_order(blockIdx.x, gridDim.x);
+    const int tile = w % ntiles, bh = w / ntiles, b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int len = length_of(a, b);
+    const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
+    const long row_base = (long)b * a.U * a.H + kvh * share;
+    const T* dout = (const T*)a.dout + row_base * a.D;
+    const int key = tile * 32 * NWK + wk * 32 + (lane & 31);
+    const bool any = tile * 32 * NWK < len;             // (workgroup-uniform)
+
+    f32x16 dk[G::NDT], dv[G::NDT];
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i) dk[i] = dv[i] = f32x16{0};
+    if (any) {
+        RowTile<T, DP, BR> tq, to;
+        float rl = INFINITY, rd = 0.f;
+        auto stats = [&](int r0) {
+            rl = INFINITY; rd = 0.f;                    // rows behind the last: p = exp2(s - inf) = 0
+            if (tid < BR && r0 + tid < R) {
+                const int u = (r0 + tid) / share, g = r0 + tid - u * share;
+                rl = a.lse[row_base + (long)u * a.H + g] - P_SHIFT<T>;
+                rd = a.delta[row_base + (long)u * a.H + g] * P_BACK;
+            }
+        };
+        tq.load_rows(q, a.q_u, a.q_h, 0, R, share, a.D, tid);
+        to.load_rows(dout, (long)a.H * a.D, a.D, 0, R, share, a.D, tid);
+        stats(0);
+        u32x4 kf[G::NCH], vf[G::NCH];
+#pragma unroll
+        for (int c = 0; c < G::NCH; ++c) {
+            kf[c] = vf[c] = u32x4{0, 0, 0, 0};
+            const int d = c * G::CH + h * G::EL;
+            if (key < len && d < a.D) {
+                kf[c] = *(const u32x4*)((const T*)a.k + b * a.k_b + kvh * a.k_h + (long)key * a.k_t + d);
+                vf[c] = *(const u32x4*)((const T*)a.v + b * a.v_b + kvh * a.v_h + (long)key * a.v_t + d);
+            }
+        }
+        for (int r0 = 0; r0 < R; r0 += BR) {
+            __syncthreads();
+            tq.store(sQ, tid);
+            to.store(sO, tid);
+            if (tid < BR) { sL[tid] = rl; sD[tid] = rd; }
+            __syncthreads();
+            if (r0 + BR < R) {
+                tq.load_rows(q, a.q_u, a.q_h, r0 + BR, R, share, a.D, tid);
+                to.load_rows(dout, (long)a.H * a.D, a.D, r0 + BR, R, share, a.D, tid);
+                stats(r0 + BR);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const int x0 = (wr * RT + t) * 32;
+                if (r0 + x0 >= R) continue;
+                f32x16 s = f32x16{0}, dp = f32x16{0};
+#pragma unroll
+                for (int c = 0; c < G::NCH; ++c) {
+                    s = Mma<T>::run(s, ld_row<T, DP>(sQ, x0 + (lane & 31), c, h), kf[c]);
+                    dp = Mma<T>::run(dp, ld_row<T, DP>(sO, x0 + (lane & 31), c, h), vf[c]);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 ls = *(const f32x4*)(sL + x0 + 8 * x + 4 * h), de = *(const f32x4*)(sD + x0 + 8 * x + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * x + e;
+                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -ls[e]));
+                        dp[r] = s[r] * fmaf(dp[r], P_BACK, -de[e]);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < G::PCH; ++c) {
+                    const u32x4 p = pack<T>(s, c), ds = pack<T>(dp, c);
+#pragma unroll
+                    for (int i = 0; i < G::NDT; ++i) {
+                        dv[i] = Mma<T>::run(dv[i], ld_t<T, DP>(sO, x0, c, i * 32, lane), p);
+                        dk[i] = Mma<T>::run(dk[i], ld_t<T, DP>(sQ, x0, c, i * 32, lane), ds);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (NWR > 1) {
+        if (any) {
+            float* red = (float*)smem;
+            auto join = [&](f32x16* acc) {
+                __syncthreads();
+                if (wr != 0) {
+#pragma unroll
+                    for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) red[(wave * DP + i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)] = acc[i][r];
+                }
+                __syncthreads();
+                if (wr == 0) {
+#pragma unroll
+                    for (int x = 1; x < NWR; ++x)
+#pragma unroll
+                        for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) acc[i][r] += red[((wave + x) * DP + i * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (lane & 31)];
+                }
+            };
+            join(dk);
+            join(dv);
+        }
+        if (wr != 0) return;
+    }
+    if (key >= a.T) return;
+    const float f = key < len ? 1.f : 0.f;
+    const long at = (((long)b * a.T + key) * a.Hkv + kvh) * a.D;
+#pragma unroll
+    for (int i = 0; i < G::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = i * 32 + 8 * x + 4 * h;
+            using V4 = __attribute__((ext_vector_type(4))) T;
+            f32x4 y = {dk[i][4 * x], dk[i][4 * x + 1], dk[i][4 * x + 2], dk[i][4 * x + 3]};
+            f32x4 z = {dv[i][4 * x], dv[i][4 * x + 1], dv[i][4 * x + 2], dv[i][4 * x + 3]};
+            if (f == 0.f) y = z = f32x4{0, 0, 0, 0};     // (a masked key's lane held whatever the zeroed operands gave)
+            if (d < a.D) {
+                *(V4*)((T*)a.dk + at + d) = __builtin_convertvector(y * a.scale, V4);
+                *(V4*)((T*)a.dv + at + d) = __builtin_convertvector(z * P_BACK, V4);
+            }
+        }
+}
+
+// ---- launch rules -----------------------------------------------------------------------------------------------------------
+constexpr int CA_CUS = 256;
+
+template <class K> int launch(K kernel, long grid, const CrossAttnArgs& a, hipStream_t stream) {
+    if (grid > 0x7fffffffL) return fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", grid);
+    if (grid == 0) return LAS_OK;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(CA_THREADS), 0, stream, a);
+    LAS_LAUNCH_CHECK();
+    return LAS_OK;
+}
+
+template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
+    const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv, n = bh * a.nsplit;
+    int rc;
+    // rows per workgroup: 128 where that still gives every CU a workgroup, else 32 with the waves side by side over the keys
+    if (R > 32 && n * ((R + 127) / 128) >= CA_CUS) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, 2>, n * ((R + 127) / 128), a, stream);
+    else rc = launch(cross_attn_fwd_kernel<T, DP, 1, 4, 1>, n * ((R + 31) / 32), a, stream);
+    if (rc != LAS_OK || a.nsplit == 1) return rc;
+    const long items = (long)a.B * a.U * a.H * (a.D / 4);
+    return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
+}
+
+template <class T, int DP> int bwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
+    const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
+    if (bh * ((R + 127) / 128) >= CA_CUS) LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 4, 1, 2>, bh * ((R + 127) / 128), a, stream));
+    else LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 1, 4, 1>, bh * ((R + 31) / 32), a, stream));
+    if (bh * ((a.T + 127) / 128) >= CA_CUS) return launch(cross_attn_dkv_kernel<T, DP, 4, 1, 2>, bh * ((a.T + 127) / 128), a, stream);
+    return launch(cross_attn_dkv_kernel<T, DP, 1, 4, 1>, bh * ((a.T + 31) / 32), a, stream);
+}
+
+template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stream) {
+    switch ((a.D + 31) / 32) {
+        case 1: return bwd ? bwd_dp<T, 32>(a, stream) : fwd_dp<T, 32>(a, stream);
+        case 2: return bwd ? bwd_dp<T, 64>(a, stream) : fwd_dp<T, 64>(a, stream);
+        case 3: return bwd ? bwd_dp<T, 96>(a, stream) : fwd_dp<T, 96>(a, stream);
+        default: return bwd ? bwd_dp<T, 128>(a, stream) : fwd_dp<T, 128>(a, stream);
+    }
+}
+
+}  // namespace
+
+// Key ranges of a forward call: as many as fill the chip twice over where the rows alone do not, none shorter than 512 keys (a range costs its
+// workgroups a partial result in fp32 and the joining launch).
+int cross_attn_splits(int B, int U, int T, int H, int Hkv) {
+    const long R = (long)U * (H / Hkv), wgs = (long)B * Hkv * ((R + 31) / 32);
+    const long want = 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / 512;
+    return (int)(want < 2 || most < 2 ? 1 : (want < most ? want : most));
+}
+
+int cross_attn(const CrossAttnArgs& a, int dtype, bool bwd, hipStream_t stream) {
+    switch (dtype) {
+        case 0: return by_dim<float>(a, bwd, stream);
+        case 1: return by_dim<__bf16>(a, bwd, stream);
+        default: return by_dim<_Float16>(a, bwd, stream);
+    }
+}
+
+}  // namespace las

@@ -1414,6 +1414,70 @@ int las_collate_pad(const float* packed_feat, const int64_t* feat_offsets, const
                        B, T, F, U, V, inputs, (long long*)targets, (hipStream_t)stream);
 }
 
+// ---------------------------------------------------------------------------------------------- cross attention
+namespace {
+
+int cross_attention_check(const las_cross_attention_desc* d, const void* q, const void* k, const void* v) {
+    LAS_REQUIRE(d, "cross attention desc");
+    LAS_REQUIRE(d->dtype >= 0 && d->dtype <= 2, "cross attention dtype");
+    LAS_REQUIRE(d->B >= 0 && d->U >= 0 && d->T >= 0 && d->H > 0 && d->Hkv > 0 && d->H % d->Hkv == 0, "cross attention dims");
+    const int el = d->dtype == 0 ? 4 : 8;
+    LAS_REQUIRE(d->D > 0 && d->D <= 128 && d->D % el == 0, "cross attention head size: at most 128 and whole 16-byte pieces");
+    LAS_REQUIRE((int64_t)d->U * (d->H / d->Hkv) < (1 << 30) && d->T < (1 << 30), "cross attention lengths");
+    const int64_t strides = d->q_b | d->q_u | d->q_h | d->k_b | d->k_t | d->k_h | d->v_b | d->v_t | d->v_h;
+    LAS_REQUIRE(strides % el == 0, "cross attention strides: multiples of 16 bytes");
+    LAS_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "cross attention rows: 16-byte aligned");
+    const bool rows = d->B > 0 && d->U > 0, keys = d->B > 0 && d->T > 0;
+    LAS_REQUIRE((!rows || q) && (!keys || (k && v)), "cross attention pointers");
+    return LAS_OK;
+}
+
+CrossAttnArgs cross_attention_args(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* lens) {
+    CrossAttnArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.lens = lens;
+    a.q_b = d->q_b; a.q_u = d->q_u; a.q_h = d->q_h; a.k_b = d->k_b; a.k_t = d->k_t; a.k_h = d->k_h; a.v_b = d->v_b; a.v_t = d->v_t; a.v_h = d->v_h;
+    a.B = d->B; a.U = d->U; a.T = d->T; a.H = d->H; a.Hkv = d->Hkv; a.D = d->D; a.nsplit = 1;
+    a.scale = d->scale; a.c = d->scale * 1.4426950408889634f;
+    return a;
+}
+
+}  // namespace
+
+size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d, int backward) {
+    if (!d || d->B <= 0 || d->U <= 0 || d->T < 0 || d->H <= 0 || d->Hkv <= 0 || d->D <= 0) return 0;
+    const size_t rows = (size_t)d->B * d->U * d->H;
+    if (backward) return rows;
+    const int n = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv);
+    return n > 1 ? rows * n * (d->D + 2) : 0;
+}
+
+int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                            void* out, float* lse, float* workspace, void* stream) {
+    LAS_TRY(cross_attention_check(d, q, k, v));
+    if (d->B == 0 || d->U == 0) return LAS_OK;
+    LAS_REQUIRE(out && ((uintptr_t)out & 15) == 0, "cross attention output");
+    CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
+    a.o = out; a.lse = lse;
+    a.nsplit = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv);
+    LAS_REQUIRE(a.nsplit == 1 || (workspace && ((uintptr_t)workspace & 15) == 0), "cross attention workspace");
+    a.part = workspace;
+    return cross_attn(a, d->dtype, false, (hipStream_t)stream);
+}
+
+int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* workspace,
+                            void* stream) {
+    LAS_TRY(cross_attention_check(d, q, k, v));
+    if (d->B == 0) return LAS_OK;
+    const bool rows = d->U > 0, keys = d->T > 0;
+    LAS_REQUIRE(!rows || (out && lse && dout && dq && workspace), "cross attention backward pointers");
+    LAS_REQUIRE(!keys || (dk && dv), "cross attention gradients");
+    LAS_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "cross attention tensors: 16-byte aligned");
+    CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
+    a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.delta = workspace;
+    return cross_attn(a, d->dtype, true, (hipStream_t)stream);
+}
+
 // ---------------------------------------------------------------------------------------------- building blocks
 int las_gemm_f32(const float* A, const float* B, float* C, const float* bias0, const float* bias1, int M, int N, int K,
                  int64_t lda, int64_t ldb, int64_t ldc, int a_kc, int b_kc, int batch, int64_t sA, int64_t sB, int64_t sC,

@@ -1,0 +1,110 @@
+"""Attention of decoder states over the Listener's features, beside ``Attention`` (one state per utterance, MLP keys): many states per
+utterance, heads of keys and values, utterances of different lengths, fp32 / bf16 / fp16 (``las_cross_attention_fwd`` / ``_bwd``)."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _cabi
+from .._cabi import CrossAttentionDesc, lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows(t, per16):
+    """``t`` itself when its rows (last dimension) are contiguous and start at multiples of 16 bytes, else a contiguous copy."""
+    sb, st, sh, sd = t.stride()
+    if sd == 1 and not (sb | st | sh) % per16 and not t.data_ptr() & 15:
+        return t
+    t = t.contiguous()
+    return t if not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check(query, key, value, key_lengths):
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if not t.is_cuda:
+            raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
+        if t.dim() != 4:
+            raise RuntimeError(f"cross_attention: {name} must be (batch, length, heads, head size), got {tuple(t.shape)}")
+        if t.dtype != query.dtype or t.device != query.device:
+            raise RuntimeError("cross_attention: query, key and value must share one type and device")
+    if query.dtype not in _DTYPES:
+        raise RuntimeError(f"cross_attention computes in fp32, bf16 or fp16; got {query.dtype}")
+    B, U, H, D = query.shape
+    if key.shape != value.shape or key.shape[0] != B or key.shape[3] != D:
+        raise RuntimeError(f"cross_attention: query {tuple(query.shape)}, key {tuple(key.shape)}, value {tuple(value.shape)} do not go together")
+    Hkv = key.shape[2]
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise RuntimeError(f"cross_attention: {H} query heads do not share {Hkv} key heads evenly")
+    per16 = 4 if query.dtype == torch.float32 else 8
+    if not 0 < D <= 128 or D % per16:
+        raise RuntimeError(f"cross_attention: the head size must be a multiple of {per16} and at most 128, got {D}")
+    if key_lengths is not None:
+        if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"cross_attention: key_lengths must be ({B},) int32 or int64, got {tuple(key_lengths.shape)} {key_lengths.dtype}")
+        if key_lengths.device != query.device:
+            raise RuntimeError("cross_attention: key_lengths must be on the device of the query")
+        if key_lengths.dtype != torch.int32:
+            key_lengths = key_lengths.clamp(0, key.shape[1]).to(torch.int32)
+        key_lengths = key_lengths.contiguous()
+    return per16, key_lengths
+
+
+def _forward(query, key, value, key_lengths, scale, per16, want_lse):
+    q, k, v = _rows(query, per16), _rows(key, per16), _rows(value, per16)
+    B, U, H, D = q.shape
+    T, Hkv = k.shape[1], k.shape[2]
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    d = CrossAttentionDesc(B, U, T, H, Hkv, D, _DTYPES[q.dtype], scale, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    out = torch.empty(B, U, H, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, U, H, device=q.device, dtype=torch.float32) if want_lse else None
+    L = lib()
+    n = L.las_cross_attention_workspace_floats(d, 0)
+    work = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+    _cabi.call_on(q.device, L.las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                  None if work is None else work.data_ptr())
+    return d, q, k, v, out, lse
+
+
+class _CrossAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, key_lengths, scale, per16):
+        d, q, k, v, out, lse = _forward(query, key, value, key_lengths, scale, per16, True)
+        ctx.save_for_backward(q, k, v, key_lengths, out, lse)
+        ctx.desc = d
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, key_lengths, out, lse = ctx.saved_tensors
+        dout = dout.contiguous()
+        if dout.data_ptr() & 15:
+            dout = dout.clone(memory_format=torch.contiguous_format)
+        dev = q.device
+        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+        dv = torch.empty(k.shape, device=dev, dtype=k.dtype)
+        delta = torch.empty(lse.shape, device=dev, dtype=torch.float32)
+        _cabi.call_on(dev, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr())
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(query, key, value, key_lengths=None, scale=None):
+    """``softmax(scale * query key^T) value`` of decoder states over an encoder's states.
+
+    ``query`` (B, U, H, D), ``key`` / ``value`` (B, T, Hkv, D) of one type (fp32, bf16, fp16), any strides; H a multiple of Hkv (query head
+    ``h`` reads key head ``h // (H // Hkv)``); D a multiple of 16 bytes, at most 128.  ``key_lengths`` (B,) int32 / int64 on the device: the
+    utterances' valid frames (clamped to [0, T]); the frames behind them are never read and get zero gradients, and an utterance without
+    any gives zeros.  ``scale`` defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once) in query, key and value.
+    Scores, softmax and sums are fp32 whatever the type.  U = 1 is one decode step: the key range is split over the GPU where the batch
+    alone does not fill it.  Rows that are not contiguous or not 16-byte aligned are copied first."""
+    per16, key_lengths = _check(query, key, value, key_lengths)
+    scale = 1.0 / math.sqrt(query.shape[3]) if scale is None else float(scale)
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        return _CrossAttentionFn.apply(query, key, value, key_lengths, scale, per16)
+    return _forward(query, key, value, key_lengths, scale, per16, False)[4]
