@@ -289,6 +289,21 @@ int las_ls_loss(const float* logp, int64_t stride_u, int64_t stride_b, const int
 int las_letter_error_rate(const float* logp, int64_t stride_u, int64_t stride_b, const int64_t* labels_onehot, int U,
                           int U_lab, int B, int V, float* ler_out, int32_t* work, void* stream);
 
+/* Distillation from a teacher's top logits, beside las_ls_loss: the row loss temperature^2 KL(softmax(teacher / temperature) over the row's K entries ||
+ * softmax(logits / temperature) over the vocabulary), averaged over an utterance's first lengths[b] steps and then over the B utterances (an
+ * utterance without steps adds nothing; steps behind lengths[b] get a zero gradient).
+ *   logits (B,U,V) of dtype 0 fp32 / 1 bf16 / 2 fp16 (log-probs are logits too), addressed logits[b*stride_b + u*stride_u + v];
+ *   index (B,U,K) int32 (index_64 = 0) or int64, teacher (B,U,K) of teacher_dtype, both contiguous, K <= 1024.  An entry whose index lies outside
+ *   [0, V) is absent, a class named twice counts with both entries, a row without entries adds nothing.
+ *   lengths int32 (B) on the device (clamped to [0, U]) or NULL: all U steps.
+ *   loss: 1 float (needs scratch: B U floats), or NULL.  dlogits: gradient of the loss in the logits' type, addressed like them with
+ *   dstride_*, or NULL; multiplied by *upstream (device) unless that is NULL.  One pass over the logits either way; no atomics. */
+int las_distill_loss(const void* logits, int64_t stride_u, int64_t stride_b, int dtype, const void* index, int index_64, const void* teacher,
+                     int teacher_dtype, const int32_t* lengths, int B, int U, int V, int K, float temperature, float* loss, void* dlogits,
+                     int64_t dstride_u, int64_t dstride_b, const float* upstream, float* scratch, void* stream);
+/* x[0..n) *= *factor (device), nothing read or written when the factor is 1: the backward of a loss whose forward left its gradient. */
+int las_scale_unless_one(void* x, size_t n, int dtype, const float* factor, void* stream);
+
 /* Global-norm clip + Adam step on the flat gradient buffer in two launches: torch.nn.utils.clip_grad_norm_(params, max_norm)
  * followed by torch.optim.Adam.step() (amsgrad off, weight_decay 0) — reference solver/solver.py:96-97, train.py:82.
  *   params[t]            device pointer of parameter tensor t (fp32, contiguous), t < n_tensors   (HOST array)

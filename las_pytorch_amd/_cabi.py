@@ -20,6 +20,8 @@ FLAG_GRADS_ZEROED = 16      # las_pblstm_bwd / las_speller_bwd: the gradient blo
 FLAG_DEFER_DW = 32          # ... their weight-gradient GEMM group may still be running on the library's side stream on return (las_join_deferred)
 FLAG_GEMM_F32 = 8           # this call's GEMMs on the fp32 matrix pipe (per call; the process-wide default is option GEMM_ARITH)
 
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # the `dtype` argument of the entry points that take several types
+
 _f = C.c_void_p   # every device pointer is passed as an integer address
 
 
@@ -93,6 +95,9 @@ PROTOTYPES = {
     "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 12),
     "las_ls_loss": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _f, _f, C.c_int64,
                               C.c_int64, _f, _f]),
+    "las_distill_loss": (C.c_int, [_f, C.c_int64, C.c_int64, C.c_int, _f, C.c_int, _f, C.c_int, _f] + [C.c_int] * 4
+                         + [C.c_float, _f, _f, C.c_int64, C.c_int64, _f, _f, _f]),
+    "las_scale_unless_one": (C.c_int, [_f, C.c_size_t, C.c_int, _f, _f]),
     "las_letter_error_rate": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, _f, _f, _f]),
     "las_collate_pad": (C.c_int, [_f, _f, _f, _f] + [C.c_int] * 5 + [_f, _f, _f]),
     "las_comm_uid": (C.c_int, [C.c_char_p]),

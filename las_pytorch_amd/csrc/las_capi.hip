@@ -1397,6 +1397,29 @@ int las_ls_loss(const float* logp, int64_t stride_u, int64_t stride_b, const int
                    dstride_u, dstride_b, (hipStream_t)stream);
 }
 
+int las_distill_loss(const void* logits, int64_t stride_u, int64_t stride_b, int dtype, const void* index, int index_64, const void* teacher,
+                     int teacher_dtype, const int32_t* lengths, int B, int U, int V, int K, float temperature, float* loss, void* dlogits,
+                     int64_t dstride_u, int64_t dstride_b, const float* upstream, float* scratch, void* stream) {
+    LAS_REQUIRE(logits && index && teacher, "distillation pointers");
+    LAS_REQUIRE(dtype >= 0 && dtype <= 2 && teacher_dtype >= 0 && teacher_dtype <= 2, "distillation dtype");
+    LAS_REQUIRE(B > 0 && U > 0 && V > 0 && V < (1 << 30) && K > 0 && K <= 1024 && (int64_t)B * U < 0x7fffffffLL, "distillation dims (1 <= K <= 1024)");
+    LAS_REQUIRE(temperature > 0.f && temperature < 1e30f, "distillation temperature: positive");
+    LAS_REQUIRE(loss || dlogits, "distillation outputs");
+    LAS_REQUIRE(!loss || scratch, "distillation scratch");
+    DistillArgs a = {};
+    a.z = logits; a.idx = index; a.t = teacher; a.dz = dlogits; a.rows = loss ? scratch : nullptr; a.lens = lengths; a.upstream = upstream;
+    a.z_b = stride_b; a.z_u = stride_u; a.dz_b = dstride_b; a.dz_u = dstride_u;
+    a.B = B; a.U = U; a.V = V; a.K = K; a.t_dtype = teacher_dtype; a.idx64 = index_64; a.tau = temperature;
+    return distill(a, dtype, loss, (hipStream_t)stream);
+}
+
+int las_scale_unless_one(void* x, size_t n, int dtype, const float* factor, void* stream) {
+    LAS_REQUIRE(dtype >= 0 && dtype <= 2, "scale dtype");
+    LAS_REQUIRE((x || n == 0) && factor, "scale pointers");
+    if (n == 0) return LAS_OK;
+    return scale_unless_one(x, n, dtype, factor, (hipStream_t)stream);
+}
+
 int las_letter_error_rate(const float* logp, int64_t stride_u, int64_t stride_b, const int64_t* labels_onehot, int U, int U_lab,
                           int B, int V, float* ler_out, int32_t* work, void* stream) {
     LAS_REQUIRE(logp && labels_onehot && ler_out, "LER pointers");      // work: unused since ABI 9 (may be NULL)

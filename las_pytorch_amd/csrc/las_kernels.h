@@ -372,4 +372,19 @@ struct CrossAttnArgs {
 int cross_attn_splits(int B, int U, int T, int H, int Hkv);
 int cross_attn(const CrossAttnArgs& a, int dtype, bool bwd, hipStream_t stream);      // dtype 0 fp32, 1 bf16, 2 fp16
 
+// ---- distill.hip -----------------------------------------------------------------------
+// Distillation from a teacher's top K logits; z (B,U,V) by strides (elements, unit stride along V), index / teacher logits (B,U,K) contiguous.
+struct DistillArgs {
+    const void *z, *idx, *t;
+    void* dz;                      // NULL: no gradient
+    float* rows;                   // B U weighted row losses; NULL: no loss
+    const int* lens;               // taught steps per utterance (clamped to [0, U]); NULL: all
+    const float* upstream;         // one factor of the gradient on the device; NULL: 1
+    long z_b, z_u, dz_b, dz_u;
+    int B, U, V, K, t_dtype, idx64;
+    float tau;
+};
+int distill(const DistillArgs& a, int dtype, float* loss, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
+int scale_unless_one(void* x, size_t n, int dtype, const float* factor, hipStream_t stream);
+
 }  // namespace las

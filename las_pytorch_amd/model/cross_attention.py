@@ -7,9 +7,7 @@ import math
 import torch
 
 from .. import _cabi
-from .._cabi import CrossAttentionDesc, lib
-
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+from .._cabi import DTYPES, CrossAttentionDesc, lib
 
 
 def _rows(t, per16):
@@ -29,7 +27,7 @@ def _check(query, key, value, key_lengths):
             raise RuntimeError(f"cross_attention: {name} must be (batch, length, heads, head size), got {tuple(t.shape)}")
         if t.dtype != query.dtype or t.device != query.device:
             raise RuntimeError("cross_attention: query, key and value must share one type and device")
-    if query.dtype not in _DTYPES:
+    if query.dtype not in DTYPES:
         raise RuntimeError(f"cross_attention computes in fp32, bf16 or fp16; got {query.dtype}")
     B, U, H, D = query.shape
     if key.shape != value.shape or key.shape[0] != B or key.shape[3] != D:
@@ -56,7 +54,7 @@ def _forward(query, key, value, key_lengths, scale, per16, want_lse):
     B, U, H, D = q.shape
     T, Hkv = k.shape[1], k.shape[2]
     qs, ks, vs = q.stride(), k.stride(), v.stride()
-    d = CrossAttentionDesc(B, U, T, H, Hkv, D, _DTYPES[q.dtype], scale, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    d = CrossAttentionDesc(B, U, T, H, Hkv, D, DTYPES[q.dtype], scale, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
     out = torch.empty(B, U, H, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, U, H, device=q.device, dtype=torch.float32) if want_lse else None
     L = lib()

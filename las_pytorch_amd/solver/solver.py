@@ -167,6 +167,98 @@ def label_smoothing_loss_backward_device(pred_y, labels_onehot_int64, label_smoo
     return loss
 
 
+class _DistillationLoss(torch.autograd.Function):
+    """``las_distill_loss``: the forward leaves the gradient of the loss beside its value (one pass over the logits), the first backward hands
+    it over, multiplied in place where its seed is not one; a further backward of a retained graph forms it again."""
+
+    @staticmethod
+    def forward(ctx, logits, index, teacher, lengths, temperature):
+        grad = torch.empty_like(logits)
+        if grad.stride(2) != 1:
+            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        loss = _distill(logits, index, teacher, lengths, temperature, True, grad, None)
+        ctx.save_for_backward(logits, index, teacher, lengths)
+        ctx.temperature, ctx.grad = temperature, grad
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, upstream):
+        from .. import _cabi
+        logits, index, teacher, lengths = ctx.saved_tensors
+        upstream = upstream.to(torch.float32).contiguous()
+        grad, ctx.grad = ctx.grad, None
+        if grad is not None:
+            _cabi.call_on(grad.device, _cabi.lib().las_scale_unless_one, grad.data_ptr(), grad.numel(), _cabi.DTYPES[grad.dtype], upstream.data_ptr())
+        else:
+            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+            _distill(logits, index, teacher, lengths, ctx.temperature, False, grad, upstream)
+        return grad, None, None, None, None
+
+
+def _distill(logits, index, teacher, lengths, temperature, want_loss, grad, upstream):
+    from .. import _cabi
+    B, U, V = logits.shape
+    K = index.shape[2]
+    dev = logits.device
+    out = torch.empty(1 + B * U, device=dev, dtype=torch.float32) if want_loss else None      # the loss, then the rows' scratch
+    at = out.data_ptr() if want_loss else None
+    gs = (0, 0) if grad is None else (grad.stride(1), grad.stride(0))
+    _cabi.call_on(dev, _cabi.lib().las_distill_loss, logits.data_ptr(), logits.stride(1), logits.stride(0), _cabi.DTYPES[logits.dtype],
+                  index.data_ptr(), int(index.dtype == torch.int64), teacher.data_ptr(), _cabi.DTYPES[teacher.dtype],
+                  None if lengths is None else lengths.data_ptr(), B, U, V, K, temperature, at, None if grad is None else grad.data_ptr(),
+                  gs[0], gs[1], None if upstream is None else upstream.data_ptr(), at + 4 if want_loss else None)
+    return out[0] if want_loss else None
+
+
+def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=1.0, lengths=None):
+    """Loss of a student against the top logits of a teacher, beside ``label_smoothing_loss_device``:
+
+        row = temperature^2 KL(softmax(teacher_logits / temperature) || softmax(pred_y / temperature)[teacher_index])
+        loss = mean_b  mean_{u < lengths[b]} row[b,u]
+
+    ``pred_y`` (B,U,V) fp32 / bf16 / fp16 logits or log-probs, any strides along B and U (the transposed view of the decode kernel's buffer
+    among them); ``teacher_index`` (B,U,K) int32 / int64 and ``teacher_logits`` (B,U,K) of any of the three types, K <= 1024: the teacher's
+    distribution is the softmax over a row's entries.  Entries with an index outside [0, V) are absent (pad shorter rows with -1); a class named twice
+    counts with both entries; a row without entries, like an utterance without steps, adds nothing.  ``lengths`` (B,) int32 / int64 on the
+    device, clamped to [0, U]; None: every step counts.  Returns a scalar fp32 tensor, differentiable (once) in ``pred_y``; its gradient has
+    the type of ``pred_y`` and is zero on steps that do not count."""
+    from .. import _cabi
+    if not pred_y.is_cuda:
+        raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
+    if pred_y.dim() != 3 or pred_y.dtype not in _cabi.DTYPES:
+        raise RuntimeError(f"distillation_loss_device: pred_y must be (B,U,V) in fp32, bf16 or fp16, got {tuple(pred_y.shape)} {pred_y.dtype}")
+    B, U, V = pred_y.shape
+    if teacher_index.dim() != 3 or teacher_index.shape[:2] != (B, U) or teacher_index.shape != teacher_logits.shape:
+        raise RuntimeError(f"distillation_loss_device: teacher_index {tuple(teacher_index.shape)} and teacher_logits {tuple(teacher_logits.shape)} must "
+                           f"both be ({B},{U},K)")
+    if teacher_index.dtype not in (torch.int32, torch.int64) or teacher_logits.dtype not in _cabi.DTYPES:
+        raise RuntimeError(f"distillation_loss_device: teacher_index must be int32 or int64 and teacher_logits fp32, bf16 or fp16, got "
+                           f"{teacher_index.dtype}, {teacher_logits.dtype}")
+    if teacher_logits.requires_grad:
+        raise RuntimeError("distillation_loss_device has no gradient for the teacher: detach teacher_logits")
+    temperature = float(temperature)
+    if not 0.0 < temperature < 1e30:
+        raise RuntimeError(f"distillation_loss_device: temperature must be positive, got {temperature}")
+    if not 1 <= teacher_index.shape[2] <= 1024 or pred_y.numel() == 0:
+        raise RuntimeError("distillation_loss_device: between 1 and 1024 teacher entries per row and at least one row are needed")
+    if lengths is not None:
+        if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"distillation_loss_device: lengths must be ({B},) int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+        if lengths.dtype != torch.int32:
+            lengths = lengths.clamp(0, U).to(torch.int32)
+        lengths = lengths.contiguous()
+    for t in (teacher_index, teacher_logits, lengths):
+        if t is not None and t.device != pred_y.device:
+            raise RuntimeError("distillation_loss_device: all tensors must be on the device of pred_y")
+    if pred_y.stride(2) != 1:
+        pred_y = pred_y.contiguous()
+    teacher_index, teacher_logits = teacher_index.contiguous(), teacher_logits.contiguous()
+    if torch.is_grad_enabled() and pred_y.requires_grad:
+        return _DistillationLoss.apply(pred_y, teacher_index, teacher_logits, lengths, temperature)
+    return _distill(pred_y, teacher_index, teacher_logits, lengths, temperature, True, None, None)
+
+
 # --------------------------------------------------------------------------------------------------
 # one step
 # --------------------------------------------------------------------------------------------------
