@@ -249,6 +249,23 @@ int las_speller_bwd(const las_speller_desc* d, const float* feat, const float* k
                     void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Drawing one token per row of logits, beside the decode modes of las_speller_fwd (which feed back their own arg-max or sample): for callers that
+ * drive las_speller_step_fwd themselves.
+ *   w = exp((logit - row maximum) / temperature), candidates in falling order of their logits, equal ones by lower index.  Kept are the first
+ *   top_k of them (<= 0: all); of those the ones before which less than top_p of their mass lies (a product in fp64; >= 1: all; the first always);
+ *   of those the ones with w >= min_p (<= 0: all).  The token is the first kept index, in vocabulary order, at which the cumulated mass
+ *   exceeds uniforms[b] times the kept mass; uniforms fp32 (B) in [0, 1) (what lies outside counts as the nearer end).
+ *   temperature <= 0 or NaN, or top_k = 1: the arg-max (lowest index), log-probability 0.
+ *   logits (B,V) of dtype 0 fp32 / 1 bf16 / 2 fp16, rows stride_b elements apart.  A NaN or -inf logit is never drawn; +inf logits share the mass; a row
+ *   of nothing else gives token -1 and log-probability -inf.
+ *   *_rows: a value per row on the device (fp32; top_k int32) in place of the scalar, or NULL.
+ *   tokens int64 (B); logprob fp32 (B) or NULL: log of the token's share of the kept mass.
+ *   Weights are formed in fp64 and summed as integers: the answer is that of the definition and does not depend on any order. */
+int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, int V, const float* uniforms, double temperature, int top_k, double top_p,
+                      double min_p, const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows,
+                      int64_t* tokens, float* logprob, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Attention of decoder states over an encoder's states of another length.  Beside las_attention_*, which attends one decoder state per
  * utterance with the reference's MLP keys (model/las_model.py:275-318): here U states per utterance, H query heads that share Hkv key /
  * value heads (H a multiple of Hkv; query head h reads head h / (H / Hkv)), and utterances of different lengths.

@@ -6,5 +6,6 @@ streams, autograd bookkeeping and ``torch.distributed``."""
 from ._cabi import check_device_errors  # noqa: F401
 from .model.cross_attention import cross_attention  # noqa: F401
 from .model.las_model import LAS, Attention, Listener, Speller, pBLSTMLayer  # noqa: F401
+from .model.sampling import sample_tokens  # noqa: F401
 
-__all__ = ["LAS", "Listener", "Speller", "Attention", "pBLSTMLayer", "cross_attention", "check_device_errors"]
+__all__ = ["LAS", "Listener", "Speller", "Attention", "pBLSTMLayer", "cross_attention", "sample_tokens", "check_device_errors"]

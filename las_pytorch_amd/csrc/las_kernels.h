@@ -387,4 +387,18 @@ struct DistillArgs {
 int distill(const DistillArgs& a, int dtype, float* loss, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
 int scale_unless_one(void* x, size_t n, int dtype, const float* factor, hipStream_t stream);
 
+// ---- sample.hip ------------------------------------------------------------------------
+// One token per row of logits (B,V).  *_rows: one value per row on the device, or NULL: the scalar.
+struct SampleArgs {
+    const void* z;
+    const float *u, *temperature_rows, *top_p_rows, *min_p_rows;
+    const int* top_k_rows;
+    long long* tokens;
+    float* logp;                   // NULL: not wanted
+    double temperature, top_p, min_p;
+    long z_b;
+    int B, V, top_k;
+};
+int sample(const SampleArgs& a, int dtype, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
+
 }  // namespace las

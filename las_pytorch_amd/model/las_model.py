@@ -25,6 +25,7 @@ import torch.nn as nn
 from .. import _cabi
 from .._cabi import (FLAG_DEFER_DW, FLAG_FORCE_GENERIC, FLAG_GRADS_ZEROED, FLAG_STASH, FLAG_TEACHER_FORCED, SpellerDesc, SpellerGrads, check, lib,
                      ptr, stream_ptr)
+from .sampling import sample_tokens
 
 def set_force_generic(module, flag=True):
     """A/B switch for tests and profiling: every pBLSTM layer / Speller under ``module`` uses the generic kernels
@@ -659,6 +660,27 @@ class Speller(nn.Module):
             h_in, c_in = last_hidden_state
         logp, h_out, c_out, ctx, att = _SpellerStepFn.apply(cfg, listener_feature, input_word.reshape(B, -1), h_in, c_in, *self._params())
         return logp, (h_out, c_out), ctx, list(att.unbind(0))
+
+
+    def sample(self, listener_feature, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Draw one sequence per utterance: ``forward_step`` in a loop (first input: symbol 0 and the first frame, as the reference's loop,
+        las_model.py:196-198), every step's symbol drawn by ``sample_tokens`` with that function's limits from ``uniforms`` (steps, B) and
+        fed back one-hot.  Returns ``(tokens (B, steps) int64, logprob (B, steps) fp32)``; no gradient.  ``temperature`` 0 follows the arg-max,
+        like ``decode_mode`` 1."""
+        steps, B = uniforms.shape
+        if listener_feature.shape[0] != B or steps < 1:
+            raise RuntimeError(f"Speller.sample: uniforms must be (steps, {listener_feature.shape[0]}), got {tuple(uniforms.shape)}")
+        with torch.no_grad():
+            symbol = torch.zeros(B, dtype=torch.int64, device=listener_feature.device)
+            context, state, tokens, logprobs = listener_feature[:, 0], None, [], []
+            for u in uniforms.unbind(0):
+                word = torch.cat([nn.functional.one_hot(symbol, self.label_dim).to(context.dtype), context], -1)
+                logits, state, context, _att = self.forward_step(word.unsqueeze(1), state, listener_feature)
+                symbol, logprob = sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+                tokens.append(symbol)
+                logprobs.append(logprob)
+                symbol = symbol.clamp_min(0)      # (-1: a row without any finite log-probability)
+            return torch.stack(tokens, 1), torch.stack(logprobs, 1)
 
 
 class LAS(nn.Module):
