@@ -260,10 +260,12 @@ int las_speller_bwd(const las_speller_desc* d, const float* feat, const float* k
  *   of nothing else gives token -1 and log-probability -inf.
  *   *_rows: a value per row on the device (fp32; top_k int32) in place of the scalar, or NULL.
  *   tokens int64 (B); logprob fp32 (B) or NULL: log of the token's share of the kept mass.
- *   Weights are formed in fp64 and summed as integers: the answer is that of the definition and does not depend on any order. */
+ *   Weights are formed in fp64 and summed as integers: the answer is that of the definition and does not depend on any order.
+ *   workspace: las_sample_workspace_bytes() bytes, 16-byte aligned (0: may be NULL), private to the call until its kernels have run. */
+size_t las_sample_workspace_bytes(int B, int V);
 int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, int V, const float* uniforms, double temperature, int top_k, double top_p,
                       double min_p, const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows,
-                      int64_t* tokens, float* logprob, void* stream);
+                      int64_t* tokens, float* logprob, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Attention of decoder states over an encoder's states of another length.  Beside las_attention_*, which attends one decoder state per

@@ -90,7 +90,8 @@ PROTOTYPES = {
     "las_speller_bwd_workspace_floats": (C.c_size_t, [C.POINTER(SpellerDesc), C.c_int]),
     "las_speller_bwd": (C.c_int, [C.POINTER(SpellerDesc), _f, _f, _f, _f, _f, C.c_int, C.c_int, _f, _f,
                                   C.POINTER(SpellerGrads), _f, C.c_int, _f]),
-    "las_sample_tokens": (C.c_int, [_f, C.c_int64, C.c_int, C.c_int, C.c_int, _f, C.c_double, C.c_int, C.c_double, C.c_double] + [_f] * 7),
+    "las_sample_tokens": (C.c_int, [_f, C.c_int64, C.c_int, C.c_int, C.c_int, _f, C.c_double, C.c_int, C.c_double, C.c_double] + [_f] * 8),
+    "las_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "las_cross_attention_workspace_floats": (C.c_size_t, [C.POINTER(CrossAttentionDesc), C.c_int]),
     "las_cross_attention_fwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 8),
     "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 12),

@@ -1438,18 +1438,21 @@ int las_collate_pad(const float* packed_feat, const int64_t* feat_offsets, const
 }
 
 // ---------------------------------------------------------------------------------------------- sampling
+size_t las_sample_workspace_bytes(int B, int V) { return B > 0 && V > 0 ? sample_workspace_bytes(B, V) : 0; }
+
 int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, int V, const float* uniforms, double temperature, int top_k, double top_p,
                       double min_p, const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows,
-                      int64_t* tokens, float* logprob, void* stream) {
+                      int64_t* tokens, float* logprob, void* workspace, void* stream) {
     LAS_REQUIRE(dtype >= 0 && dtype <= 2, "sampling dtype");
-    LAS_REQUIRE(B >= 0 && V > 0 && V < (1 << 30), "sampling dims");
+    LAS_REQUIRE(B >= 0 && B < (1 << 30) && V > 0 && V < (1 << 30), "sampling dims");
     if (B == 0) return LAS_OK;
     LAS_REQUIRE(logits && uniforms && tokens, "sampling pointers");
     SampleArgs a = {};
     a.z = logits; a.z_b = stride_b; a.B = B; a.V = V; a.u = uniforms; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
     a.temperature_rows = temperature_rows; a.top_k_rows = top_k_rows; a.top_p_rows = top_p_rows; a.min_p_rows = min_p_rows;
     a.tokens = (long long*)tokens; a.logp = logprob;
-    return sample(a, dtype, (hipStream_t)stream);
+    LAS_REQUIRE(sample_workspace_bytes(B, V) == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "sampling workspace");
+    return sample(a, dtype, workspace, (hipStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------------------------- cross attention

@@ -399,6 +399,9 @@ struct SampleArgs {
     long z_b;
     int B, V, top_k;
 };
-int sample(const SampleArgs& a, int dtype, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
+constexpr int SM_SLICES = 64;      // most slices of a row
+int sample_slices(int B, int V);
+size_t sample_workspace_bytes(int B, int V);      // 0: none
+int sample(const SampleArgs& a, int dtype, void* workspace, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
 
 }  // namespace las

@@ -7,9 +7,13 @@
 // The answer is a whole number that hangs on borders of long sums, so the sums are exact: w is formed in fp64 and held as an integer multiple of
 // 2^-s (s = 62 - bits of V, at most 50), and integers add to the same sum in any order — by atomics too.  All three limits keep a head of the
 // falling order, so the kept set is "every candidate not behind one cut", and the cut is one 64-bit number: (order-preserving bits of the logit,
-// inverted index).  Cuts are found without sorting: a histogram of the distance to the maximum finds the bin that holds the cut, the candidates
-// down to that bin go to a list in LDS, and the list is searched digit by digit.  Where a bin holds more than the list, the same search runs
-// over the row itself.
+// inverted index).  Cuts are found without sorting the row: a histogram of the distance to the maximum finds the bin that holds the cut, the
+// candidates down to that bin go to a list, and only the list is sorted.  Where a bin holds more than the list can, the cut is searched digit by
+// digit over the row itself.
+//
+// One workgroup works at a row where rows alone fill the GPU; otherwise a row is cut into slices (a workgroup each) in four launches: slice
+// maxima, histogram, candidates and slice masses, the draw.  (Letting the row's last workgroup of the third draw at once was measured: its fences
+// write back and drop whole L2s, 139 us at 64 rows of 32000 where that launch now takes a few and the fourth 10.)
 #include "las_common.h"
 #include "las_kernels.h"
 #include <math.h>
@@ -19,18 +23,25 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SM_BINS = 2048, SM_CAP = 4096;
-constexpr float SM_RANGE = 51.f;                 // log2 units below the maximum: what lies further weighs nothing (s <= 50)
+constexpr int SM_BINS = 2048, SM_CAP = 4096, SM_TABLE = 256;
+constexpr double SM_RANGE = 51.0;                // log2 units below the maximum: what lies further weighs nothing (s <= 50)
 
-template <class T> static __device__ __forceinline__ float logit_at(const T* z, long i) {
-    const float x = (float)z[i];
+template <class T> static __device__ __forceinline__ float clean(T v) {
+    const float x = (float)v;
     return x == x ? x + 0.f : -INFINITY;         // NaN is never drawn; -0 and +0 are one logit
 }
+template <class T> static __device__ __forceinline__ float logit_at(const T* z, int i) { return clean(z[i]); }
 
-static __device__ __forceinline__ u64 place(float z, int i) {        // falling order of candidates = falling order of these numbers
+static __device__ __forceinline__ u64 place_of(float z, int i) {     // falling order of candidates = falling order of these numbers
     const unsigned b = __float_as_uint(z), k = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (u64)k << 32 | (unsigned)~i;
 }
+static __device__ __forceinline__ float logit_of(u64 place) {
+    const unsigned k = (unsigned)(place >> 32);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+static __device__ __forceinline__ int index_of(u64 place) { return (int)~(unsigned)place; }
+static __device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
 
 // floor(u n) for 0 < u < 1, exactly: 24 bits of u times 64 bits of n
 static __device__ __forceinline__ u64 floor_of_product(float u, u64 n) {
@@ -41,55 +52,194 @@ static __device__ __forceinline__ u64 floor_of_product(float u, u64 n) {
     return shift >= 128 ? 0 : shift >= 64 ? hi >> (shift - 64) : lo >> shift | hi << (64 - shift);
 }
 
-// What one row needs to weigh a logit.
+// 2^d for d <= 0 in fp64: 2^(j / 256) from a table, the remainder (at most 1/512 away) by the exponential's series to the fourth power (the fifth is
+// below 4e-17), the whole part by the exponent.  A third of the instructions of the library's exp2, which a row of 10^5 logits feels.
 struct Weigher {
+    const double* table;       // 2^(j / SM_TABLE)
     double a, unit;            // log2(e) / T, 2^s
     float zmax, af;            // bins per logit
-    __device__ __forceinline__ double weight(float z) const { return z == zmax ? 1.0 : exp2(((double)z - (double)zmax) * a); }
-    __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double2ull_rn(w * unit); }
+    __device__ __forceinline__ u64 fixed(float z) const {
+        const double d = z == zmax ? 0.0 : fmax(((double)z - (double)zmax) * a, -256.0);
+        const double r = __builtin_rint(d * SM_TABLE);
+        const int j = (int)r;
+        const double f = fma(r, -1.0 / SM_TABLE, d);
+        const double p = f * fma(f, fma(f, fma(f, 0.009618129107628477, 0.05550410866482158), 0.2402265069591007), 0.6931471805599453);
+        const double t = table[j & (SM_TABLE - 1)];
+        return rounded(ldexp(fma(t, p, t), j >> 8) * unit);
+    }
+    static __device__ __forceinline__ u64 rounded(double x) {        // to the nearest integer, 0 <= x <= 2^50
+        return (u64)__double_as_longlong(x + 4503599627370496.0) & 0xfffffffffffffull;
+    }
     __device__ __forceinline__ int bin(float z) const {               // 0 at the maximum, monotone in z
         if (z == zmax) return 0;
         const float y = (zmax - z) * af;
         return y < (float)(SM_BINS - 1) ? (int)y : SM_BINS - 1;
     }
 };
+static_assert(SM_TABLE == 256, "Weigher::fixed takes the low eight bits");
 
+struct Limits {
+    double temperature, top_p, min_p;
+    long top_k;
+    float u;
+    __device__ __forceinline__ Limits(const SampleArgs& a, int row) {
+        temperature = a.temperature_rows ? (double)a.temperature_rows[row] : a.temperature;
+        top_k = a.top_k_rows ? (long)a.top_k_rows[row] : (long)a.top_k;
+        top_p = a.top_p_rows ? (double)a.top_p_rows[row] : a.top_p;
+        min_p = a.min_p_rows ? (double)a.min_p_rows[row] : a.min_p;
+        u = a.u[row];
+    }
+    __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0) || top_k == 1; }
+    __device__ __forceinline__ bool by_count(int V) const { return top_k > 1 && top_k < V; }
+    __device__ __forceinline__ bool by_mass() const { return top_p < 1.0; }
+    // the head's mass: the first candidate at which the sum reaches this is the last that top_p keeps
+    __device__ __forceinline__ u64 head(u64 total) const {
+        const u64 g = top_p > 0.0 ? (u64)ceil(top_p * (double)total) : 1;
+        return g < 1 ? (u64)1 : g > total ? total : g;
+    }
+    // cumulated > u total  <=>  cumulated >= floor(u total) + 1
+    __device__ __forceinline__ u64 goal(u64 total) const { return u >= 1.f ? total : (u > 0.f ? floor_of_product(u, total) : 0) + 1; }
+    __device__ __forceinline__ u64 least(double unit) const { return min_p > 0.0 ? Weigher::rounded(fmin(min_p, 1.0) * unit) : 0; }
+};
+
+static __device__ __forceinline__ Weigher weigher(const double* table, float zmax, double temperature, int V) {
+    Weigher w;
+    w.table = table;
+    w.zmax = zmax;
+    w.a = 1.4426950408889634 / temperature;
+    w.unit = (double)(1ull << min(50, 62 - (32 - __clz(V))));
+    w.af = (float)(w.a * ((SM_BINS - 1) / SM_RANGE));
+    return w;
+}
+
+static __device__ __forceinline__ void fill_table(double* table, int tid, int nt) {
+    for (int i = tid; i < SM_TABLE; i += nt) table[i] = exp2((double)i / SM_TABLE);
+}
+
+static __device__ __forceinline__ void answer(const SampleArgs& a, int row, int token, float logp) {
+    a.tokens[row] = token;
+    if (a.logp) a.logp[row] = logp;
+}
+static __device__ __forceinline__ float share(u64 part, u64 total) { return (float)log((double)part / (double)total); }
+
+// ---- one wave ---------------------------------------------------------------------------------------------------------------
+static __device__ __forceinline__ u64 wave_sum(u64 x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+static __device__ __forceinline__ u64 wave_scan(u64 x) {             // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(x, o); if (lane >= o) x += y; }
+    return x;
+}
+// falling order over the wave
+static __device__ __forceinline__ u64 wave_sort(u64 x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const u64 y = __shfl_xor(x, o);
+            const bool want_large = ((lane & o) == 0) == ((lane & size) == 0);
+            x = want_large == (x > y) ? x : y;
+        }
+    return x;
+}
+
+// All candidates that can be kept, one per lane (0: none), drawn from by one wave.  w: of the row's maximum.
+// head: the mass that top_p keeps, where the list is the head of a longer row (0: the list is all that top_k left, or all there is).
+static __device__ __forceinline__ void wave_draw(const SampleArgs& a, int row, const Limits& lim, const Weigher& w, u64 mine, u64 head) {
+    const int lane = threadIdx.x & 63;
+    u64 p = wave_sort(mine);
+    u64 x = p ? w.fixed(logit_of(p)) : 0;
+    if (lim.by_count(a.V) && lane >= lim.top_k) x = p = 0;
+    if (lim.by_mass()) {
+        const u64 incl = wave_scan(x), total = __shfl(incl, 63);
+        if (incl - x >= (head ? head : lim.head(total))) x = p = 0;
+    }
+    if (x < lim.least(w.unit)) x = p = 0;
+    // vocabulary order: lowest index first = largest inverted index first (a dropped candidate's 0 goes last)
+    p = wave_sort(p << 32 | p >> 32);
+    x = p ? w.fixed(logit_of(p << 32 | p >> 32)) : 0;
+    const u64 incl = wave_scan(x), total = __shfl(incl, 63), goal = lim.goal(total);
+    if (incl - x < goal && goal <= incl) answer(a, row, (int)~(unsigned)(p >> 32), share(x, total));
+}
+
+// ---- one workgroup ----------------------------------------------------------------------------------------------------------
 struct Shared {
     u64 mass[SM_BINS];
     unsigned count[SM_BINS];
     u64 place[SM_CAP];
-    u64 weight[SM_CAP];
+    double table[SM_TABLE];
     u64 red[32];
     u64 out[4];
-    float fred[32];
     unsigned n;
 };
 
 template <int NT> static __device__ __forceinline__ u64 block_sum(u64 x, Shared& s) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    if constexpr (NT == 64) return x;
+    x = wave_sum(x);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = x;
     __syncthreads();
     x = 0;
+#pragma unroll
     for (int i = 0; i < NT / 64; ++i) x += s.red[i];
     return x;
 }
+template <int NT> static __device__ __forceinline__ u64 block_max(u64 x, Shared& s) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = larger(x, __shfl_xor(x, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = x;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) x = larger(x, s.red[i]);
+    return x;
+}
+// inclusive, and the sum over all
+template <int NT> static __device__ __forceinline__ u64 block_scan(u64 x, u64& total, Shared& s) {
+    x = wave_scan(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) s.red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    total = 0;
+    const int wave = threadIdx.x >> 6;
+    u64 before = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) { const u64 y = s.red[i]; if (i < wave) before += y; total += y; }
+    return x + before;
+}
+// falling order over the workgroup, one number per thread; buf: NT numbers
+template <int NT> static __device__ __forceinline__ u64 block_sort(u64 x, u64* buf) {
+    const int tid = threadIdx.x;
+    for (int size = 2; size <= NT; size <<= 1)
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            u64 y;
+            if (o >= 64) {
+                __syncthreads();
+                buf[tid] = x;
+                __syncthreads();
+                y = buf[tid ^ o];
+            } else {
+                y = __shfl_xor(x, o);
+            }
+            const bool want_large = ((tid & o) == 0) == ((tid & size) == 0);
+            x = want_large == (x > y) ? x : y;
+        }
+    return x;
+}
 
-// The first entry of a table of n (n <= NT * PER) at which the running sum reaches `target` (>= 1, reached somewhere): (entry, sum before it).
+// The first entry of a table of n at which the running sum reaches `target` (>= 1, at most the table's sum): (entry, sum before it).
 template <int NT, class At> static __device__ __forceinline__ void reach(int n, u64 target, At at, Shared& s, int& entry, u64& before) {
     const int tid = threadIdx.x, per = (n + NT - 1) / NT, lo = min(n, tid * per), hi = min(n, lo + per);
     u64 mine = 0;
     for (int i = lo; i < hi; ++i) mine += at(i);
-    u64 incl = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(incl, o); if ((tid & 63) >= o) incl += y; }
-    __syncthreads();
-    if ((tid & 63) == 63) s.red[tid >> 6] = incl;
+    u64 total;
+    const u64 incl = block_scan<NT>(mine, total, s);
     if (tid == 0) { s.out[0] = (u64)(n - 1); s.out[1] = 0; }      // (an entry of the table whatever the target)
     __syncthreads();
-    for (int i = 0; i < (tid >> 6); ++i) incl += s.red[i];
     u64 run = incl - mine;
     if (run < target && target <= incl) {
         for (int i = lo; i < hi; ++i) {
@@ -104,16 +254,16 @@ template <int NT, class At> static __device__ __forceinline__ void reach(int n, 
     __syncthreads();
 }
 
-// The number at which the running sum of `value` over the numbers, largest first, reaches target: eight bits at a time.
+// The number at which the running sum of `value` over the numbers, largest first, reaches target: eight bits at a time, `bits` of them.
 // each(f): calls f(number, value) for this thread's share of the candidates.
-template <int NT, class Each> static __device__ __forceinline__ u64 search(u64 target, Each each, Shared& s) {
+template <int NT, class Each> static __device__ __forceinline__ u64 search(u64 target, int bits, Each each, Shared& s) {
     u64 found = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int shift = bits - 8; shift >= 0; shift -= 8) {
         __syncthreads();
         for (int i = threadIdx.x; i < 256; i += NT) s.mass[i] = 0;
         __syncthreads();
         each([&](u64 number, u64 value) {
-            if (shift == 56 || (number >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&s.mass[255 - ((number >> shift) & 255)], value);
+            if (shift == bits - 8 || (number >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&s.mass[255 - ((number >> shift) & 255)], value);
         });
         __syncthreads();
         int digit; u64 before;
@@ -124,229 +274,444 @@ template <int NT, class Each> static __device__ __forceinline__ u64 search(u64 t
     return found;
 }
 
-template <class T, int NT>
-__global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
-    __shared__ Shared s;
-    const int tid = threadIdx.x, row = blockIdx.x, V = a.V;
-    const T* z = (const T*)a.z + row * a.z_b;
-    const double temperature = a.temperature_rows ? (double)a.temperature_rows[row] : a.temperature;
-    const long k_arg = a.top_k_rows ? (long)a.top_k_rows[row] : (long)a.top_k;
-    const double top_p = a.top_p_rows ? (double)a.top_p_rows[row] : a.top_p;
-    const double min_p = a.min_p_rows ? (double)a.min_p_rows[row] : a.min_p;
-    const float u = a.u[row];
-
-    // the maximum and its first place
-    u64 best = 0;
-    for (int i = tid; i < V; i += NT) { const u64 p = place(logit_at(z, i), i); best = best > p ? best : p; }
+// f(logit, index) for this thread's share of [lo, hi) of a row, sixteen bytes at a time
+template <int NT, class T, class F> static __device__ __forceinline__ void each_logit(const T* z, int lo, int hi, F f) {
+    constexpr int EL = 16 / (int)sizeof(T);
+    typedef T V __attribute__((ext_vector_type(EL), aligned(sizeof(T))));
+    for (int i = lo + (int)threadIdx.x * EL; i < hi; i += NT * EL) {
+        if (i + EL <= hi) {
+            const V x = *(const V*)(z + i);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const u64 y = __shfl_xor(best, o); best = best > y ? best : y; }
-    if constexpr (NT > 64) {
-        if ((tid & 63) == 0) s.red[tid >> 6] = best;
-        __syncthreads();
-        for (int i = 0; i < NT / 64; ++i) best = best > s.red[i] ? best : s.red[i];
-        __syncthreads();
+            for (int e = 0; e < EL; ++e) f(clean((T)x[e]), i + e);
+        } else {
+            for (int e = i; e < hi; ++e) f(logit_at(z, e), e);
+        }
     }
-    const int first = (int)~(unsigned)best;
-    const float zmax = logit_at(z, first);
-    auto answer = [&](int token, float logp) {
-        a.tokens[row] = token;
-        if (a.logp) a.logp[row] = logp;
+}
+
+// Every candidate that can be kept is in s.place[0 .. n): draw.  head: see wave_draw.
+template <int NT> static __device__ void draw_listed(const SampleArgs& a, int row, const Limits& lim, const Weigher& w, int n, u64 head, Shared& s) {
+    const int tid = threadIdx.x;
+    if (n <= 64) {
+        if (tid < 64) wave_draw(a, row, lim, w, tid < n ? s.place[tid] : 0, head);
+        return;
+    }
+    if (n <= NT) {
+        u64* buf = s.mass;                        // (NT <= SM_BINS)
+        u64 total;
+        u64 p = block_sort<NT>(tid < n ? s.place[tid] : 0, buf);
+        u64 x = p ? w.fixed(logit_of(p)) : 0;
+        if (lim.by_count(a.V) && tid >= lim.top_k) x = p = 0;
+        if (lim.by_mass()) {
+            const u64 incl = block_scan<NT>(x, total, s);
+            if (incl - x >= (head ? head : lim.head(total))) x = p = 0;
+        }
+        if (x < lim.least(w.unit)) x = p = 0;
+        p = block_sort<NT>(p << 32 | p >> 32, buf);
+        x = p ? w.fixed(logit_of(p << 32 | p >> 32)) : 0;
+        const u64 incl = block_scan<NT>(x, total, s), goal = lim.goal(total);
+        if (incl - x < goal && goal <= incl) answer(a, row, (int)~(unsigned)(p >> 32), share(x, total));
+        return;
+    }
+    auto each = [&](auto f) { for (int i = tid; i < n; i += NT) f(s.place[i], w.fixed(logit_of(s.place[i]))); };
+    u64 cut = 0, m = 0;
+    if (lim.by_count(a.V)) cut = search<NT>((u64)min(lim.top_k, (long)n), 64, [&](auto f) { each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
+    if (lim.by_mass()) {
+        each([&](u64 p, u64 x) { if (p >= cut) m += x; });
+        const u64 total = block_sum<NT>(m, s);
+        cut = search<NT>(head ? head : lim.head(total), 64, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut) f(p, x); }); }, s);
+    }
+    const u64 least = lim.least(w.unit);
+    m = 0;
+    each([&](u64 p, u64 x) { if (p >= cut && x >= least) m += x; });
+    const u64 total = block_sum<NT>(m, s);
+    const u64 at = search<NT>(lim.goal(total), 32, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut && x >= least) f((u64)(unsigned)p, x); }); }, s);
+    const int token = (int)~(unsigned)at;
+    each([&](u64 p, u64 x) { if (index_of(p) == token) answer(a, row, token, share(x, total)); });
+}
+
+// The cut in a list of the candidates of one bin: the one at which the running sum (of masses, or of candidates) reaches target.
+template <int NT> static __device__ __forceinline__ u64 cut_in_list(const Weigher& w, bool masses, u64 target, int n, Shared& s) {
+    const int tid = threadIdx.x;
+    if (n <= NT) {
+        u64 total;
+        const u64 p = block_sort<NT>(tid < n ? s.place[tid] : 0, s.mass), x = p ? (masses ? w.fixed(logit_of(p)) : 1) : 0;
+        const u64 incl = block_scan<NT>(x, total, s);
+        __syncthreads();
+        if (incl - x < target && target <= incl) s.out[2] = p;
+        __syncthreads();
+        return s.out[2];
+    }
+    return search<NT>(target, 64, [&](auto f) {
+        for (int i = tid; i < n; i += NT) f(s.place[i], masses ? w.fixed(logit_of(s.place[i])) : (u64)1);
+    }, s);
+}
+
+// The draw within [lo, hi) of a row, of the candidates not behind the cut: target as in reach, total for the share.  Ranges of the range, one per
+// wave, until every thread has one index.
+template <int NT, class T>
+static __device__ void draw_range(const SampleArgs& a, int row, const T* z, const Weigher& w, u64 cut, u64 least, int lo, int hi, u64 target, u64 total, Shared& s) {
+    constexpr int NW = NT / 64;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    auto mass_at = [&](int i) {
+        const float x = logit_at(z, i);
+        if (x == -INFINITY || place_of(x, i) < cut) return (u64)0;
+        const u64 f = w.fixed(x);
+        return f >= least ? f : (u64)0;
     };
-    if (zmax == -INFINITY) { if (tid == 0) answer(-1, -INFINITY); return; }        // nothing to draw from
-    if (!(temperature > 0.0) || k_arg == 1) { if (tid == 0) answer(first, 0.f); return; }
+    while (hi - lo > NT) {
+        const int per = (hi - lo + NW - 1) / NW, x0 = min(hi, lo + wave * per), x1 = min(hi, x0 + per);
+        u64 m = 0;
+        for (int i = x0 + lane; i < x1; i += 64) m += mass_at(i);
+        m = wave_sum(m);
+        __syncthreads();
+        if (lane == 0) s.mass[wave] = m;
+        __syncthreads();
+        int part; u64 before;
+        reach<NT>(NW, target, [&](int i) { return s.mass[i]; }, s, part, before);
+        target -= before;
+        lo = min(hi, lo + part * per);
+        hi = min(hi, lo + per);
+    }
+    const u64 x = lo + tid < hi ? mass_at(lo + tid) : 0;
+    u64 all;
+    const u64 incl = block_scan<NT>(x, all, s);
+    if (incl - x < target && target <= incl) answer(a, row, lo + tid, share(x, total));
+}
 
-    Weigher w;
-    w.zmax = zmax;
-    w.a = 1.4426950408889634 / temperature;
-    const int bits = 32 - __clz(V);
-    w.unit = (double)(1ull << min(50, 62 - bits));
-    w.af = (float)(w.a * ((SM_BINS - 1) / (double)SM_RANGE));
+// ---- the row in one workgroup -----------------------------------------------------------------------------------------------
+// The cut over the whole row, for bins that hold more than a list can.
+template <int NT, class T> static __device__ __forceinline__ u64 cut_in_row(const T* z, int V, const Weigher& w, u64 cut, bool masses, u64 target, Shared& s) {
+    return search<NT>(target, 64, [&](auto f) {
+        each_logit<NT>(z, 0, V, [&](float x, int i) {
+            if (x == -INFINITY) return;
+            const u64 p = place_of(x, i);
+            if (p >= cut) f(p, masses ? w.fixed(x) : (u64)1);
+        });
+    }, s);
+}
+
+template <class T, int NT> static __device__ void row_draw(const SampleArgs& a, int row, const T* z, const Limits& lim, const Weigher& w, Shared& s) {
+    const int tid = threadIdx.x, V = a.V;
     u64 cut = 0;                                  // kept: place >= cut
-    bool listed = false;                          // the list holds every kept candidate
-    int n = 0;
 
-    auto gather = [&](int lo, int hi) {           // candidates of bins lo..hi that are not behind the cut
+    auto gather = [&](int lo, int hi) {           // candidates of bins lo..hi that are not behind the cut; their number
         __syncthreads();
         if (tid == 0) s.n = 0;
         __syncthreads();
-        for (int i = tid; i < V; i += NT) {
-            const float x = logit_at(z, i);
-            if (x == -INFINITY) continue;
+        each_logit<NT>(z, 0, V, [&](float x, int i) {
+            if (x == -INFINITY) return;
             const int b = w.bin(x);
-            const u64 p = place(x, i);
-            if (b < lo || b > hi || p < cut) continue;
+            const u64 p = place_of(x, i);
+            if (b < lo || b > hi || p < cut) return;
             const unsigned at = atomicAdd(&s.n, 1u);
-            if (at < SM_CAP) { s.place[at] = p; s.weight[at] = w.fixed(w.weight(x)); }
-        }
+            if (at < SM_CAP) s.place[at] = p;
+        });
         __syncthreads();
-        n = min((int)s.n, SM_CAP);
-        __syncthreads();
+        return min((int)s.n, SM_CAP);
     };
-    auto list_each = [&](auto f) { for (int i = tid; i < n; i += NT) f(s.place[i], s.weight[i]); };
-    auto row_each = [&](auto f) {
-        for (int i = tid; i < V; i += NT) {
-            const float x = logit_at(z, i);
-            if (x == -INFINITY) continue;
-            const u64 p = place(x, i);
-            if (p >= cut) f(p, w.fixed(w.weight(x)));
-        }
-    };
-    // counts (by_mass: masses too) of the candidates not behind the cut, by bin
-    auto histogram = [&](bool by_mass) {
+    // counts (masses too) of the candidates not behind the cut, by bin; the number of all
+    auto histogram = [&](bool masses) {
         __syncthreads();
         for (int i = tid; i < SM_BINS; i += NT) { s.mass[i] = 0; s.count[i] = 0; }
         __syncthreads();
-        for (int i = tid; i < V; i += NT) {
-            const float x = logit_at(z, i);
-            if (x == -INFINITY || place(x, i) < cut) continue;
+        each_logit<NT>(z, 0, V, [&](float x, int i) {
+            if (x == -INFINITY || place_of(x, i) < cut) return;
             const int b = w.bin(x);
             atomicAdd(&s.count[b], 1u);
-            if (by_mass) atomicAdd(&s.mass[b], w.fixed(w.weight(x)));
-        }
+            if (masses) atomicAdd(&s.mass[b], w.fixed(x));
+        });
         __syncthreads();
-    };
-    auto counted = [&](int bin) {                 // candidates before the bin
         u64 c = 0;
-        for (int i = tid; i < bin; i += NT) c += s.count[i];
+        for (int i = tid; i < SM_BINS; i += NT) c += s.count[i];
         return block_sum<NT>(c, s);
     };
 
-    if (k_arg > 1 && k_arg < V) {
-        histogram(false);
-        u64 c = 0;
-        for (int i = tid; i < SM_BINS; i += NT) c += s.count[i];
-        const u64 all = block_sum<NT>(c, s);
-        if ((u64)k_arg < all) {
+    if (lim.by_count(V)) {
+        if ((u64)lim.top_k < histogram(false)) {
             int bin; u64 before;
-            reach<NT>(SM_BINS, (u64)k_arg, [&](int i) { return (u64)s.count[i]; }, s, bin, before);
+            reach<NT>(SM_BINS, (u64)lim.top_k, [&](int i) { return (u64)s.count[i]; }, s, bin, before);
             const unsigned here = s.count[bin];
-            if (before + here <= SM_CAP) {
-                gather(0, bin);
-                listed = true;
-                cut = search<NT>((u64)k_arg, [&](auto f) { list_each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
-            } else if (here <= SM_CAP) {
-                gather(bin, bin);
-                cut = search<NT>((u64)k_arg - before, [&](auto f) { list_each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
-            } else {
-                cut = search<NT>((u64)k_arg, [&](auto f) { row_each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
-            }
+            if (before + here <= SM_CAP) return draw_listed<NT>(a, row, lim, w, gather(0, bin), 0, s);
+            if (here <= SM_CAP) cut = cut_in_list<NT>(w, false, (u64)lim.top_k - before, gather(bin, bin), s);
+            else cut = cut_in_row<NT>(z, V, w, 0, false, (u64)lim.top_k, s);
         }
     }
-    if (top_p < 1.0) {
-        auto goal = [&](u64 total) {              // the head's mass: the first candidate at which the sum reaches top_p of the total is the last kept
-            const double t = top_p > 0.0 ? ceil(top_p * (double)total) : 1.0;
-            const u64 g = (u64)t;
-            return g < 1 ? (u64)1 : g > total ? total : g;
-        };
-        if (listed) {
-            u64 m = 0;
-            list_each([&](u64 p, u64 x) { if (p >= cut) m += x; });
-            const u64 total = block_sum<NT>(m, s);
-            cut = search<NT>(goal(total), [&](auto f) { list_each([&](u64 p, u64 x) { if (p >= cut) f(p, x); }); }, s);
-        } else {
-            histogram(true);
-            u64 m = 0;
-            for (int i = tid; i < SM_BINS; i += NT) m += s.mass[i];
-            const u64 target = goal(block_sum<NT>(m, s));
-            int bin; u64 before;
-            reach<NT>(SM_BINS, target, [&](int i) { return s.mass[i]; }, s, bin, before);
-            const unsigned here = s.count[bin];
-            const u64 head = counted(bin);
-            if (head + here <= SM_CAP) {
-                gather(0, bin);
-                listed = true;
-                cut = search<NT>(target, [&](auto f) { list_each([&](u64 p, u64 x) { f(p, x); }); }, s);
-            } else if (here <= SM_CAP) {
-                gather(bin, bin);
-                cut = search<NT>(target - before, [&](auto f) { list_each([&](u64 p, u64 x) { f(p, x); }); }, s);
-            } else {
-                cut = search<NT>(target, row_each, s);
-            }
-        }
+    if (lim.by_mass()) {
+        histogram(true);
+        u64 m = 0;
+        for (int i = tid; i < SM_BINS; i += NT) m += s.mass[i];
+        const u64 target = lim.head(block_sum<NT>(m, s));
+        int bin; u64 before;
+        reach<NT>(SM_BINS, target, [&](int i) { return s.mass[i]; }, s, bin, before);
+        const unsigned here = s.count[bin];
+        u64 ahead = 0;
+        for (int i = tid; i < bin; i += NT) ahead += s.count[i];
+        ahead = block_sum<NT>(ahead, s);
+        if (cut == 0 && ahead + here <= NT) return draw_listed<NT>(a, row, lim, w, gather(0, bin), target, s);
+        if (here <= SM_CAP) cut = cut_in_list<NT>(w, true, target - before, gather(bin, bin), s);
+        else cut = cut_in_row<NT>(z, V, w, cut, true, target, s);
     }
-
-    // the draw: mass of the kept candidates, then the first index at which the cumulated mass exceeds u of it
-    const u64 least = min_p > 0.0 ? w.fixed(fmin(min_p, 1.0)) : 0;
-    auto goal = [&](u64 total) {                  // cumulated > u total  <=>  cumulated >= floor(u total) + 1
-        if (u >= 1.f) return total;
-        return (u > 0.f ? floor_of_product(u, total) : 0) + 1;
-    };
-    auto keeps = [&](u64 p, u64 x) { return p >= cut && x >= least; };
-    u64 total = 0;
-    int token;
-    if (listed) {
-        list_each([&](u64 p, u64 x) { if (keeps(p, x)) total += x; });
-        total = block_sum<NT>(total, s);
-        // lowest index first: the inverted index, largest first
-        const u64 at = search<NT>(goal(total), [&](auto f) { list_each([&](u64 p, u64 x) { if (keeps(p, x)) f((u64)(unsigned)p, x); }); }, s);
-        token = (int)~(unsigned)at;
-    } else {
-        // ranges of the row, one per wave, then ranges of the range that holds the target, until every thread has one index
-        constexpr int NW = NT / 64;
-        const int wave = tid >> 6, lane = tid & 63;
-        int lo = 0, hi = V;
-        u64 target = 0;
-        bool first_level = true;
-        while (true) {
-            const int per = hi - lo <= NT ? 0 : (hi - lo + NW - 1) / NW;
-            if (per == 0) break;
-            const int x0 = min(hi, lo + wave * per), x1 = min(hi, x0 + per);
-            u64 m = 0;
-            for (int i = x0 + lane; i < x1; i += 64) {
-                const float x = logit_at(z, i);
-                if (x == -INFINITY) continue;
-                const u64 f = w.fixed(w.weight(x));
-                if (keeps(place(x, i), f)) m += f;
-            }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o);
-            __syncthreads();
-            if (lane == 0) s.mass[wave] = m;
-            __syncthreads();
-            if (first_level) {
-                for (int i = 0; i < NW; ++i) total += s.mass[i];
-                target = goal(total);
-                first_level = false;
-            }
-            int part; u64 before;
-            reach<NT>(NW, target, [&](int i) { return s.mass[i]; }, s, part, before);
-            target -= before;
-            const int next = min(hi, lo + part * per);
-            hi = min(hi, next + per);
-            lo = next;
-        }
-        u64 mine = 0;
-        if (lo + tid < hi) {
-            const float x = logit_at(z, lo + tid);
-            if (x != -INFINITY) {
-                const u64 f = w.fixed(w.weight(x));
-                if (keeps(place(x, lo + tid), f)) mine = f;
-            }
-        }
-        __syncthreads();
-        s.weight[tid] = mine;
-        if (first_level) { total = block_sum<NT>(mine, s); target = goal(total); }
-        __syncthreads();
-        int at; u64 before;
-        reach<NT>(NT, target, [&](int i) { return s.weight[i]; }, s, at, before);
-        token = lo + at;
-    }
-    if (tid == 0) answer(token, (float)log((double)w.fixed(w.weight(logit_at(z, token))) / (double)total));
+    const u64 least = lim.least(w.unit);
+    u64 m = 0;
+    each_logit<NT>(z, 0, V, [&](float x, int i) {
+        if (x == -INFINITY || place_of(x, i) < cut) return;
+        const u64 f = w.fixed(x);
+        if (f >= least) m += f;
+    });
+    const u64 total = block_sum<NT>(m, s);
+    draw_range<NT>(a, row, z, w, cut, least, 0, V, lim.goal(total), total, s);
 }
 
-template <class T, int NT> int launch(const SampleArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((sample_kernel<T, NT>), dim3((unsigned)a.B), dim3(NT), 0, stream, a);
+template <class T, int NT> __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
+    __shared__ Shared s;
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const T* z = (const T*)a.z + row * a.z_b;
+    const Limits lim(a, row);
+    u64 best = 0;
+    each_logit<NT>(z, 0, a.V, [&](float x, int i) { best = larger(best, place_of(x, i)); });
+    best = block_max<NT>(best, s);
+    const float zmax = logit_of(best);
+    if (zmax == -INFINITY) { if (tid == 0) answer(a, row, -1, -INFINITY); return; }        // nothing to draw from
+    if (lim.greedy()) { if (tid == 0) answer(a, row, index_of(best), 0.f); return; }
+    fill_table(s.table, tid, NT);
+    __syncthreads();
+    row_draw<T, NT>(a, row, z, lim, weigher(s.table, zmax, lim.temperature, a.V), s);
+}
+
+// rows of at most 64 logits: a wave each
+constexpr int SW_THREADS = 256;
+template <class T> __global__ __launch_bounds__(SW_THREADS) void sample_wave_kernel(SampleArgs a) {
+    __shared__ double table[SM_TABLE];
+    fill_table(table, threadIdx.x, SW_THREADS);
+    __syncthreads();
+    const int row = blockIdx.x * (SW_THREADS / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= a.B) return;
+    const Limits lim(a, row);
+    const float x = lane < a.V ? logit_at((const T*)a.z + row * a.z_b, lane) : -INFINITY;
+    u64 best = lane < a.V ? place_of(x, lane) : 0;
+    const u64 mine = x > -INFINITY ? best : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = larger(best, __shfl_xor(best, o));
+    const float zmax = logit_of(best);
+    if (zmax == -INFINITY) { if (lane == 0) answer(a, row, -1, -INFINITY); return; }
+    if (lim.greedy()) { if (lane == 0) answer(a, row, index_of(best), 0.f); return; }
+    wave_draw(a, row, lim, weigher(table, zmax, lim.temperature, a.V), mine, 0);
+}
+
+// ---- the row in slices ------------------------------------------------------------------------------------------------------
+constexpr int SL_THREADS = 512;
+
+// How a row is drawn once its histogram is known: LISTED every candidate that can be kept goes to the list, CUT only those of the bin of the cut
+// (the bins before it are kept whole), WHOLE everything is kept, ALONE a bin is longer than the list: one workgroup takes the row by itself.
+enum Mode : int { LISTED, CUT, WHOLE, ALONE };
+
+// workspace of one row
+struct RowSpace {
+    u64 mass[SM_BINS];
+    unsigned count[SM_BINS];
+    u64 place[SM_CAP];
+    u64 slice_max[SM_SLICES], slice_mass[SM_SLICES];
+    u64 target, head;              // of the first slice's verdict: mass to reach within the bin, mass that top_p keeps
+    int mode;
+    unsigned n;
+};
+
+static __device__ __forceinline__ void slice_of(int V, int S, int i, int& lo, int& hi) {
+    const int per = ((V + S - 1) / S + 7) & ~7;
+    lo = min(V, i * per);
+    hi = min(V, lo + per);
+}
+
+template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_max_kernel(SampleArgs a, RowSpace* space, int S) {
+    __shared__ u64 red[SL_THREADS / 64];
+    const int tid = threadIdx.x, row = blockIdx.x / S, slice = blockIdx.x - row * S;
+    RowSpace& r = space[row];
+    for (int i = slice * SL_THREADS + tid; i < SM_BINS; i += S * SL_THREADS) { r.mass[i] = 0; r.count[i] = 0; }
+    if (slice == 0 && tid == 0) r.n = 0;
+    int lo, hi;
+    slice_of(a.V, S, slice, lo, hi);
+    u64 best = 0;
+    each_logit<SL_THREADS>((const T*)a.z + row * a.z_b, lo, hi, [&](float x, int i) { best = larger(best, place_of(x, i)); });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = larger(best, __shfl_xor(best, o));
+    if ((tid & 63) == 0) red[tid >> 6] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < SL_THREADS / 64; ++i) best = larger(best, red[i]);
+        r.slice_max[slice] = best;
+    }
+}
+
+static __device__ __forceinline__ u64 row_max(const RowSpace& r, int S, Shared& s) {
+    return block_max<SL_THREADS>((int)threadIdx.x < S ? r.slice_max[threadIdx.x] : 0, s);
+}
+
+template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_histogram_kernel(SampleArgs a, RowSpace* space, int S) {
+    __shared__ Shared s;
+    const int tid = threadIdx.x, row = blockIdx.x / S, slice = blockIdx.x - row * S;
+    RowSpace& r = space[row];
+    const Limits lim(a, row);
+    const bool masses = !lim.by_count(a.V);      // (with top_k the first cut is one of counts)
+    const float zmax = logit_of(row_max(r, S, s));
+    if (zmax == -INFINITY || lim.greedy() || (!lim.by_count(a.V) && !lim.by_mass())) return;
+    fill_table(s.table, tid, SL_THREADS);
+    for (int i = tid; i < SM_BINS; i += SL_THREADS) { s.mass[i] = 0; s.count[i] = 0; }
+    __syncthreads();
+    const Weigher w = weigher(s.table, zmax, lim.temperature, a.V);
+    int lo, hi;
+    slice_of(a.V, S, slice, lo, hi);
+    each_logit<SL_THREADS>((const T*)a.z + row * a.z_b, lo, hi, [&](float x, int) {
+        if (x == -INFINITY) return;
+        const int b = w.bin(x);
+        atomicAdd(&s.count[b], 1u);
+        if (masses) atomicAdd(&s.mass[b], w.fixed(x));
+    });
+    __syncthreads();
+    for (int i = tid; i < SM_BINS; i += SL_THREADS)
+        if (s.count[i]) { atomicAdd(&r.count[i], s.count[i]); if (masses) atomicAdd(&r.mass[i], s.mass[i]); }
+}
+
+template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_slice_kernel(SampleArgs a, RowSpace* space, int S) {
+    constexpr int NT = SL_THREADS;
+    __shared__ Shared s;
+    const int tid = threadIdx.x, row = blockIdx.x / S, slice = blockIdx.x - row * S, V = a.V;
+    RowSpace& r = space[row];
+    const Limits lim(a, row);
+    const T* z = (const T*)a.z + row * a.z_b;
+    const u64 best = row_max(r, S, s);
+    const float zmax = logit_of(best);
+    const bool first = slice == 0 && tid == 0;
+    if (zmax == -INFINITY || lim.greedy()) return;
+    fill_table(s.table, tid, NT);
+    __syncthreads();
+    const Weigher w = weigher(s.table, zmax, lim.temperature, V);
+    const u64 least = lim.least(w.unit);
+
+    // every slice comes to the same verdict
+    int mode = WHOLE, bin = SM_BINS;
+    u64 target = 0, head = 0;
+    if (lim.by_count(V) || lim.by_mass()) {
+        u64 c = 0, m = 0;
+        for (int i = tid; i < SM_BINS; i += NT) { s.count[i] = r.count[i]; s.mass[i] = r.mass[i]; c += s.count[i]; m += s.mass[i]; }
+        const u64 all = block_sum<NT>(c, s), mass = block_sum<NT>(m, s);
+        u64 before;
+        if (lim.by_count(V)) {
+            if ((u64)lim.top_k < all) {
+                reach<NT>(SM_BINS, (u64)lim.top_k, [&](int i) { return (u64)s.count[i]; }, s, bin, before);
+                mode = before + s.count[bin] <= SM_CAP ? LISTED : ALONE;
+            } else {
+                mode = lim.by_mass() ? ALONE : WHOLE;      // (fewer candidates than top_k: no masses were counted)
+            }
+        } else {
+            target = head = lim.head(mass);
+            reach<NT>(SM_BINS, target, [&](int i) { return s.mass[i]; }, s, bin, before);
+            target -= before;
+            u64 ahead = 0;
+            for (int i = tid; i < bin; i += NT) ahead += s.count[i];
+            ahead = block_sum<NT>(ahead, s);
+            const unsigned here = s.count[bin];
+            mode = ahead + here <= NT ? LISTED : here <= SM_CAP ? CUT : ALONE;
+        }
+    }
+    if (first) { r.mode = mode; r.target = target; r.head = head; }
+    if (mode == ALONE) return;
+    int lo, hi;
+    slice_of(V, S, slice, lo, hi);
+    u64 m = 0;
+    each_logit<NT>(z, lo, hi, [&](float x, int i) {
+        if (x == -INFINITY) return;
+        const int b = w.bin(x);
+        if (b > bin) return;
+        if (mode == LISTED || b == bin) {
+            const unsigned at = atomicAdd(&r.n, 1u);
+            if (at < SM_CAP) r.place[at] = place_of(x, i);
+        } else {
+            const u64 f = w.fixed(x);
+            if (f >= least) m += f;
+        }
+    });
+    if (mode == LISTED) return;
+    m = block_sum<NT>(m, s);
+    if (tid == 0) r.slice_mass[slice] = m;
+}
+
+template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_draw_kernel(SampleArgs a, const RowSpace* space, int S) {
+    constexpr int NT = SL_THREADS;
+    __shared__ Shared s;
+    __shared__ u64 masses[SM_SLICES];
+    const int tid = threadIdx.x, row = blockIdx.x, V = a.V;
+    const RowSpace& r = space[row];
+    const Limits lim(a, row);
+    const T* z = (const T*)a.z + row * a.z_b;
+    const u64 best = row_max(r, S, s);
+    const float zmax = logit_of(best);
+    if (zmax == -INFINITY) { if (tid == 0) answer(a, row, -1, -INFINITY); return; }
+    if (lim.greedy()) { if (tid == 0) answer(a, row, index_of(best), 0.f); return; }
+    fill_table(s.table, tid, NT);
+    const Weigher w = weigher(s.table, zmax, lim.temperature, V);
+    const u64 least = lim.least(w.unit);
+    const int mode = r.mode, n = mode == LISTED || mode == CUT ? min((int)r.n, SM_CAP) : 0;
+    for (int i = tid; i < n; i += NT) s.place[i] = r.place[i];
+    if (tid < S) masses[tid] = r.slice_mass[tid];
+    __syncthreads();
+    if (mode == ALONE) return row_draw<T, NT>(a, row, z, lim, w, s);
+    if (mode == LISTED) return draw_listed<NT>(a, row, lim, w, n, r.head, s);
+    u64 cut = 0;
+    if (mode == CUT) {
+        cut = cut_in_list<NT>(w, true, r.target, n, s);
+        const int per = ((V + S - 1) / S + 7) & ~7;
+        for (int i = tid; i < n; i += NT) {
+            const u64 p = s.place[i];
+            if (p < cut) continue;
+            const u64 f = w.fixed(logit_of(p));
+            if (f >= least) atomicAdd(&masses[index_of(p) / per], f);
+        }
+        __syncthreads();
+    }
+    const u64 total = block_sum<NT>(tid < S ? masses[tid] : 0, s), goal = lim.goal(total);
+    u64 before;
+    int part, lo, hi;
+    reach<NT>(S, goal, [&](int i) { return masses[i]; }, s, part, before);
+    slice_of(V, S, part, lo, hi);
+    draw_range<NT>(a, row, z, w, cut, least, lo, hi, goal - before, total, s);
+}
+
+template <class T> int by_size(const SampleArgs& a, void* workspace, hipStream_t stream) {
+    const int S = sample_slices(a.B, a.V);
+    if (a.V <= 64) {
+        hipLaunchKernelGGL(sample_wave_kernel<T>, dim3((unsigned)((a.B + 3) / 4)), dim3(SW_THREADS), 0, stream, a);
+    } else if (S > 1) {
+        const dim3 grid((unsigned)(a.B * S));
+        RowSpace* space = (RowSpace*)workspace;
+        hipLaunchKernelGGL(sample_max_kernel<T>, grid, dim3(SL_THREADS), 0, stream, a, space, S);
+        // (limits that differ by row are known on the device alone: the histogram's workgroups leave at once where a row needs none)
+        if (a.top_k_rows || a.top_p_rows || (a.top_k > 1 && a.top_k < a.V) || a.top_p < 1.0)
+            hipLaunchKernelGGL(sample_histogram_kernel<T>, grid, dim3(SL_THREADS), 0, stream, a, space, S);
+        hipLaunchKernelGGL(sample_slice_kernel<T>, grid, dim3(SL_THREADS), 0, stream, a, space, S);
+        hipLaunchKernelGGL(sample_draw_kernel<T>, dim3((unsigned)a.B), dim3(SL_THREADS), 0, stream, a, space, S);
+    } else if (a.V <= 4096) {
+        hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3((unsigned)a.B), dim3(256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3((unsigned)a.B), dim3(1024), 0, stream, a);
+    }
     LAS_LAUNCH_CHECK();
     return LAS_OK;
-}
-template <class T> int by_size(const SampleArgs& a, hipStream_t stream) {
-    return a.V <= 4096 ? launch<T, 256>(a, stream) : launch<T, 1024>(a, stream);
 }
 
 }  // namespace
 
-int sample(const SampleArgs& a, int dtype, hipStream_t stream) {
-    return dtype == 0 ? by_size<float>(a, stream) : dtype == 1 ? by_size<__bf16>(a, stream) : by_size<_Float16>(a, stream);
+// Slices of a row: the GPU's 256 CUs twice over shared among the rows, no slice shorter than 4096 logits.  One (a workgroup per row, no workspace) where
+// that leaves no more than one.
+int sample_slices(int B, int V) {
+    const int want = B > 0 ? 512 / B : 1, most = V / 4096;
+    const int S = want < most ? want : most;
+    return S < 2 ? 1 : S > SM_SLICES ? SM_SLICES : S;
+}
+size_t sample_workspace_bytes(int B, int V) { return V > 64 && sample_slices(B, V) > 1 ? (size_t)B * sizeof(RowSpace) : 0; }
+
+int sample(const SampleArgs& a, int dtype, void* workspace, hipStream_t stream) {
+    return dtype == 0 ? by_size<float>(a, workspace, stream) : dtype == 1 ? by_size<__bf16>(a, workspace, stream) : by_size<_Float16>(a, workspace, stream);
 }
 
 }  // namespace las

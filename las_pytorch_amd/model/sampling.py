@@ -57,6 +57,9 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     uniforms = uniforms.contiguous()
     tokens = torch.empty(B, device=dev, dtype=torch.int64)
     logprob = torch.empty(B, device=dev, dtype=torch.float32)
-    _cabi.call_on(dev, lib().las_sample_tokens, logits.data_ptr(), logits.stride(0), DTYPES[logits.dtype], B, V, uniforms.data_ptr(), t, min(k, 2 ** 31 - 1), p, m,
-                  tr, kr, pr, mr, tokens.data_ptr(), logprob.data_ptr())
+    L = lib()
+    n = L.las_sample_workspace_bytes(B, V)
+    work = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    _cabi.call_on(dev, L.las_sample_tokens, logits.data_ptr(), logits.stride(0), DTYPES[logits.dtype], B, V, uniforms.data_ptr(), t, min(k, 2 ** 31 - 1), p, m,
+                  tr, kr, pr, mr, tokens.data_ptr(), logprob.data_ptr(), None if work is None else work.data_ptr())
     return tokens, logprob

@@ -252,11 +252,12 @@ def test_refusals():
 def test_c_entry_refuses_before_it_launches():
     """Status 1 and a message, nothing touched (runs without a GPU)."""
     L = _cabi.lib()
-    good = dict(z=4096, sb=8, dtype=0, B=1, V=8, u=4096, t=1.0, k=0, p=1.0, m=0.0, tr=None, kr=None, pr=None, mr=None, tokens=4096, logp=None, stream=None)
-    for change in (dict(z=None), dict(u=None), dict(tokens=None), dict(dtype=3), dict(dtype=-1), dict(B=-1), dict(V=0), dict(V=1 << 30)):
+    good = dict(z=4096, sb=8, dtype=0, B=1, V=8, u=4096, t=1.0, k=0, p=1.0, m=0.0, tr=None, kr=None, pr=None, mr=None, tokens=4096, logp=None, work=None, stream=None)
+    for change in (dict(z=None), dict(u=None), dict(tokens=None), dict(dtype=3), dict(dtype=-1), dict(B=-1), dict(V=0), dict(V=1 << 30), dict(V=1 << 16)):
         assert L.las_sample_tokens(*{**good, **change}.values()) == 1, change
         assert b"sampling" in L.las_last_error()
     assert L.las_sample_tokens(*{**good, "B": 0}.values()) == 0
+    assert L.las_sample_workspace_bytes(1, 1 << 16) > 0 and L.las_sample_workspace_bytes(1, 64) == 0 and L.las_sample_workspace_bytes(1000, 1 << 16) == 0
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         sample_tokens(torch.zeros(2, 5), torch.zeros(2))
 
