@@ -71,10 +71,14 @@ template <class T> static __device__ __forceinline__ u32x4 pack(const f32x16& x,
     }
 }
 
-// fp16 keeps its full precision only above 2^-14: probabilities are formed 2^14 times too large there (at most 2^14 of 65504; a power of two in
-// the exponential's argument costs nothing) and the sums divided by it, so that a probability is good to half a step down to 2^-28.
+// fp16 keeps its full precision only above 2^-14: probabilities are formed 2^P_SHIFT times too large there (a power of two in the exponential's
+// argument costs nothing) and the sums divided by it: by 2^14 in the backward, where none exceeds one (2^14 of 65504), by 2^9 in the forward, where
+// the running maximum may lag by 2^P_SLACK.
 template <class T> constexpr float P_SHIFT = 0.f;
+template <class T> constexpr float P_SHIFT_FWD = 0.f;
 template <> constexpr float P_SHIFT<_Float16> = 14.f;
+template <> constexpr float P_SHIFT_FWD<_Float16> = 9.f;
+constexpr float P_SLACK = 6.f;
 
 // left operand, row-major: chunk c of row `row` of an LDS tile
 template <class T, int DP> static __device__ __forceinline__ u32x4 ld_row(const T* s, int row, int c, int h) {
@@ -141,7 +145,8 @@ template <class T, int DP, int ROWS> struct RowTile {
 static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
 // Workgroups of one (utterance, key head) read the same keys: give each XCD (blockIdx % 8 on this device) a contiguous run of work so that
-// they share its L2.  A permutation of [0, n) for any n: correct whatever the placement.
+// they share its L2.  A permutation of [0, n) for any n: correct whatever the placement.  The order runs over utterances first, then heads: an
+// XCD's run then mixes long and short utterances.
 static __device__ __forceinline__ int xcd_order(int b, int n) {
     const int per = n >> 3, rem = n & 7, x = b & 7, i = b >> 3;
     return x * per + min(x, rem) + i;
@@ -151,10 +156,14 @@ static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
     return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
 }
 
+// Workgroups per CU that the registers are budgeted for (as many waves per SIMD): two where a workgroup's tiles fit 256 registers, else one.
+template <class T, int DP> constexpr int FWD_PER_CU = sizeof(T) == 2 || DP <= 32 ? 2 : 1;
+template <class T, int DP> constexpr int BWD_PER_CU = (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1;
+
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 // Four waves: NWQ of them side by side over rows (32 each), NWK over keys (KT tiles of 32 of every key tile each).
 template <class T, int DP, int NWQ, int NWK, int KT>
-__global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fwd_kernel(CrossAttnArgs a) {
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
     constexpr int RED = NWK > 1 ? 4 * (DP + 2) * 32 * 4 : 0;                    // bytes of the joining of waves
@@ -165,7 +174,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArg
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
     const int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = w % ntiles, split = (w / ntiles) % a.nsplit, bh = w / (ntiles * a.nsplit), b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int tile = w % ntiles, split = (w / ntiles) % a.nsplit, bh = w / (ntiles * a.nsplit), b = bh % a.B, kvh = bh / a.B;
     const int len = length_of(a, b);
     const int per = ((len + a.nsplit - 1) / a.nsplit + 31) & ~31;
     const int begin = min(len, split * per), end = min(len, begin + per);
@@ -222,7 +231,9 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArg
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
         mx = fmaxf(m, fmaxf(mx, other_half(mx)));
-        if (__any(mx > m)) {
+        // The maximum only has to keep the exponentials in range: it follows the true one when that has grown by more than 2^P_SLACK somewhere in the
+        // wave, which is once or twice in a row of any length, not at almost every tile.
+        if (__any((mx - m) * a.c > P_SLACK)) {
             const float alpha = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mx) * a.c);
             l *= alpha;
 #pragma unroll
@@ -231,7 +242,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArg
                 for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
             m = mx;
         }
-        const float mc = (m == -INFINITY ? 0.f : m * a.c) - P_SHIFT<T>;
+        const float mc = (m == -INFINITY ? 0.f : m * a.c) - P_SHIFT_FWD<T>;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
 #pragma unroll
@@ -309,7 +320,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_fwd_kernel(CrossAttnArg
             const f32x4 y = {acc[i][4 * x] * inv, acc[i][4 * x + 1] * inv, acc[i][4 * x + 2] * inv, acc[i][4 * x + 3] * inv};
             if (d < a.D) *(V4*)(o + d) = __builtin_convertvector(y, V4);
         }
-    if (a.lse && h == 0) a.lse[out_row] = l > 0.f ? fmaf(m, a.c, log2f(l) - P_SHIFT<T>) : (l == 0.f ? -INFINITY : l);
+    if (a.lse && h == 0) a.lse[out_row] = l > 0.f ? fmaf(m, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
 }
 
 // joins the key ranges of a split forward: four values of one row per thread
@@ -336,13 +347,13 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnAr
     using V4 = __attribute__((ext_vector_type(4))) T;
     acc *= inv;
     *(V4*)((T*)a.o + row * a.D + d) = __builtin_convertvector(acc, V4);
-    if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT<T>) : (l == 0.f ? -INFINITY : l);
+    if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
 }
 
 // ---- backward: dq (and D_i) -------------------------------------------------------------------------------------------------
 // The forward's shape: one row per lane; q and do stay in registers, every key tile is read once per row tile.
 template <class T, int DP, int NWQ, int NWK, int KT>
-__global__ __launch_bounds__(CA_THREADS) void cross_attn_dq_kernel(CrossAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq_kernel(CrossAttnArgs a) {
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
     constexpr int RED = NWK > 1 ? 4 * DP * 32 * 4 : 0;
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_dq_kernel(CrossAttnArgs
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
     const int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = w % ntiles, bh = w / ntiles, b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
     const int end = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
@@ -455,7 +466,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_dq_kernel(CrossAttnArgs
 // ---- backward: dk, dv -------------------------------------------------------------------------------------------------------
 // One key per lane (k and v in registers), row tiles of q and do through LDS; NWK waves side by side over keys, NWR over rows.
 template <class T, int DP, int NWK, int NWR, int RT>
-__global__ __launch_bounds__(CA_THREADS) void cross_attn_dkv_kernel(CrossAttnArgs a) {
+__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dkv_kernel(CrossAttnArgs a) {
     using G = Geo<T, DP>;
     constexpr int BR = 32 * RT * NWR;
     constexpr float P_BACK = P_SHIFT<T> == 0.f ? 1.f : 1.f / 16384.f;
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_dkv_kernel(CrossAttnArg
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
     const int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = w % ntiles, bh = w / ntiles, b = bh / a.Hkv, kvh = bh % a.Hkv;
+    const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
     const int len = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const long row_base = (long)b * a.U * a.H + kvh * share;

@@ -7,7 +7,7 @@ probabilities and absolute values taken inside every sum:
   out  h |out| + (h + e + T 2^-24) sum_j P |v|                        (P rounded to the type, T-term sum, output rounded)
   ds   h |ds| + P (E_dp + E_D) + e P (|dp| + |D|),  E_dp = D 2^-24 |do||v|,  E_D = (h + D 2^-24) sum |do||out|  (D from the rounded out)
   fp16 only: what is rounded to it below 2^-14 is off by up to half a subnormal step, 2^-25 (``sub``): each ds; each P, which the kernels form
-       2^14 times too large, by 2^-39 of the row's largest (forward) or of 1 (backward)
+       too large, by 2^9 in the forward, 2^14 in the backward: by 2^-34 of the row's largest (P is taken relative to a maximum of the row's scores), 2^-39
   dq, dk, dv: the type's half step of the result plus those errors times the other factor, plus the sum's own length times 2^-24."""
 import math
 
@@ -41,7 +41,7 @@ def reference(q, k, v, lengths, dout=None, scale=None):
     out = P @ V
     absP = scale * Q.abs() @ K.abs().transpose(2, 3)
     rel = (2 * ((D + 4) * f32 * absP.amax(-1, keepdim=True) if T else 0.0) + 8 * f32)
-    E_out = (h + f32) * out.abs() + (h + rel + T * f32) * (P @ V.abs()) + sub * 2.0 ** -14 * V.abs().sum(2, keepdim=True)
+    E_out = (h + f32) * out.abs() + (h + rel + T * f32) * (P @ V.abs()) + sub * 2.0 ** -9 * V.abs().sum(2, keepdim=True)
     back = lambda x: x.permute(0, 2, 1, 3)      # noqa: E731
     res = {"out": (back(out), back(E_out))}
     if dout is None:
