@@ -193,12 +193,25 @@ def stream_ptr():
 
 def call_on(device, fn, *args):
     """``check(fn(*args, stream))`` with ``device`` current and its current stream: a launch goes to the device that is current, whatever its
-    operands live on."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    operands live on.  (The raw queries: ``torch.cuda.current_device`` / ``current_stream`` cost more than the launch itself.)"""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc)
+
+
+def differentiable_once(backward):
+    """``torch.autograd.function.once_differentiable`` for a backward that calls the library, without its bookkeeping where no graph of the
+    backward is asked for (the ordinary case)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 _err_words = {}

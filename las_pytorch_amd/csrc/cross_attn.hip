@@ -12,7 +12,7 @@
 // between the wave's halves, the rescale factor is one value per lane, and the probabilities leave the matrix instruction in just
 // the shape that the second product wants as its right operand once the keys are taken in the order in which they lie in registers
 // (a contraction may take its index in any order, if both operands do).  The left operand of that product (V^T, and K^T / Q^T / dO^T in
-// the backward) is read from the row-major tile by the transposing LDS load for 16-bit types, by plain dword loads for fp32.
+// the backward) is read from the row-major tile by the transposing LDS load.
 #include "las_common.h"
 #include "las_kernels.h"
 #include <math.h>
@@ -28,47 +28,96 @@ using s16x4 = __attribute__((ext_vector_type(4))) short;
 
 constexpr int CA_THREADS = 256;
 
-// ---- the matrix instruction by type: one 16-byte chunk per lane of either operand -------------------------------------------
-// 16-bit: one 32x32x16 (lane half h holds contraction indices 8 h .. 8 h + 7 of 16).  fp32: four 32x32x2 (index 4 h + j of 8 in step j).
-template <class T> struct Mma;
-template <> struct Mma<__bf16> {
-    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mma<_Float16> {
-    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mma<float> {
-    static __device__ __forceinline__ f32x16 run(f32x16 c, u32x4 a, u32x4 b) {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
-        return c;
-    }
-};
+// ---- operands by type ------------------------------------------------------------------------------------------------------
+// Every product runs on the 32x32x16 16-bit matrix instruction (lane half h holds contraction indices 8 h .. 8 h + 7 of 16; accumulation in fp32).
+// A fp32 operand is the exact sum of three bf16 terms (x1 = rne(x), x2 = rne(x - x1), x3 = x - x1 - x2); six of the nine partial products are
+// formed, the other three are below 2^-26 of |a b|: the accuracy of the fp32 matrix instruction at 2.67 times its rate, as in the GEMM.  (An infinite
+// operand becomes NaN on the way: inf - inf.)  The terms of a tile lie in three planes of LDS, split once per workgroup as they are stored.
+template <class T> struct Term { using E = T; static constexpr int N = 1; };
+template <> struct Term<float> { using E = __bf16; static constexpr int N = 3; };
 
-// geometry of one type: EL elements per 16-byte chunk, a chunk of both lane halves covers CH contraction indices
+// eight contraction indices of one lane, all terms
+template <class T> struct Frag { u32x4 p[Term<T>::N]; };
+
+static __device__ __forceinline__ f32x16 mma16(f32x16 c, u32x4 a, u32x4 b, __bf16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+static __device__ __forceinline__ f32x16 mma16(f32x16 c, u32x4 a, u32x4 b, _Float16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <class T> static __device__ __forceinline__ f32x16 mma(f32x16 c, const Frag<T>& a, const Frag<T>& b) {
+    using E = typename Term<T>::E;
+    if constexpr (Term<T>::N == 3) {
+        c = mma16(c, a.p[0], b.p[2], E{});
+        c = mma16(c, a.p[2], b.p[0], E{});
+        c = mma16(c, a.p[1], b.p[1], E{});
+        c = mma16(c, a.p[0], b.p[1], E{});
+        c = mma16(c, a.p[1], b.p[0], E{});
+    }
+    return mma16(c, a.p[0], b.p[0], E{});
+}
+
+// eight fp32 values as an operand.  16-bit types: rounding P and dS to the inputs' type costs half a step (2^-9 bf16, 2^-12 fp16) per term of sums
+// that stay in fp32.
+template <class T> static __device__ __forceinline__ Frag<T> frag_of(f32x8 x) {
+    using V8 = __attribute__((ext_vector_type(8))) typename Term<T>::E;
+    Frag<T> f;
+    if constexpr (Term<T>::N == 3) {
+        const V8 a = __builtin_convertvector(x, V8);
+        x -= __builtin_convertvector(a, f32x8);
+        const V8 b = __builtin_convertvector(x, V8);
+        x -= __builtin_convertvector(b, f32x8);
+        f.p[0] = __builtin_bit_cast(u32x4, a);
+        f.p[1] = __builtin_bit_cast(u32x4, b);
+        f.p[2] = __builtin_bit_cast(u32x4, __builtin_convertvector(x, V8));
+    } else {
+        f.p[0] = __builtin_bit_cast(u32x4, __builtin_convertvector(x, V8));
+    }
+    return f;
+}
+
+// geometry: a row of DP elements is CPR sixteen-byte pieces of EL elements in global memory and LD elements (a piece of padding: rows start four banks
+// apart) in a plane of LDS; NCH chunks of 16 contraction indices, NDT accumulator tiles
 template <class T, int DP> struct Geo {
-    static constexpr int EL = 16 / (int)sizeof(T), CH = 2 * EL, NCH = DP / CH, LD = DP + EL, CPR = DP / EL, NDT = DP / 32;
-    static constexpr int PCH = 32 / CH;        // chunks of a 32-row contraction
+    static constexpr int EL = 16 / (int)sizeof(T), CPR = DP / EL, LD = DP + 8, NCH = DP / 16, NDT = DP / 32;
+    static constexpr int plane(int rows) { return rows * LD; }
+    static constexpr int bytes(int rows) { return plane(rows) * 2 * Term<T>::N; }
 };
 
-// chunk c of the 32x32 accumulator tile as the right operand of the next product: accumulator register r of lane half h is row
-// 8 (r / 4) + 4 h + r % 4, so a 16-bit chunk (registers 8 c .. 8 c + 7) holds rows 16 c + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} and a
-// fp32 chunk (registers 4 c .. 4 c + 3) rows 8 c + 4 h .. + 3.  ld_t below reads the left operand in the same order.
-// Rounding P and dS to the inputs' 16 bits costs half a step (2^-9 bf16, 2^-12 fp16) per term of sums that stay in fp32.
-template <class T> static __device__ __forceinline__ u32x4 pack(const f32x16& x, int c) {
+// eight elements of a row in global memory from element d on (zeros from `D` on), as fp32 values or as an operand
+template <class T> static __device__ __forceinline__ f32x8 values_at(const T* row, int d, int D) {
+    f32x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
     if constexpr (sizeof(T) == 4) {
-        f32x4 y = {x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-        return __builtin_bit_cast(u32x4, y);
+        if (d < D) { const f32x4 y = *(const f32x4*)(row + d); x[0] = y[0]; x[1] = y[1]; x[2] = y[2]; x[3] = y[3]; }
+        if (d + 4 < D) { const f32x4 y = *(const f32x4*)(row + d + 4); x[4] = y[0]; x[5] = y[1]; x[6] = y[2]; x[7] = y[3]; }
     } else {
         using V8 = __attribute__((ext_vector_type(8))) T;
-        f32x8 y = {x[8 * c], x[8 * c + 1], x[8 * c + 2], x[8 * c + 3], x[8 * c + 4], x[8 * c + 5], x[8 * c + 6], x[8 * c + 7]};
-        return __builtin_bit_cast(u32x4, __builtin_convertvector(y, V8));
+        if (d < D) x = __builtin_convertvector(*(const V8*)(row + d), f32x8);
     }
+    return x;
+}
+template <class T> static __device__ __forceinline__ Frag<T> frag_at(const T* row, int d, int D) {
+    if constexpr (sizeof(T) == 4) {
+        return frag_of<T>(values_at(row, d, D));
+    } else {
+        Frag<T> f;
+        f.p[0] = u32x4{0, 0, 0, 0};
+        if (d < D) f.p[0] = *(const u32x4*)(row + d);
+        return f;
+    }
+}
+template <class T> static __device__ __forceinline__ Frag<T> no_frag() {
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < Term<T>::N; ++i) f.p[i] = u32x4{0, 0, 0, 0};
+    return f;
+}
+
+// chunk c (0, 1) of the 32x32 accumulator tile as the right operand of the next product: accumulator register r of lane half h is row
+// 8 (r / 4) + 4 h + r % 4, so registers 8 c .. 8 c + 7 hold rows 16 c + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}.  ld_t below reads the left operand in
+// the same order.
+template <class T> static __device__ __forceinline__ Frag<T> pack(const f32x16& x, int c) {
+    return frag_of<T>(f32x8{x[8 * c], x[8 * c + 1], x[8 * c + 2], x[8 * c + 3], x[8 * c + 4], x[8 * c + 5], x[8 * c + 6], x[8 * c + 7]});
 }
 
 // fp16 keeps its full precision only above 2^-14: probabilities are formed 2^P_SHIFT times too large there (a power of two in the exponential's
@@ -80,37 +129,41 @@ template <> constexpr float P_SHIFT<_Float16> = 14.f;
 template <> constexpr float P_SHIFT_FWD<_Float16> = 9.f;
 constexpr float P_SLACK = 6.f;
 
-// left operand, row-major: chunk c of row `row` of an LDS tile
-template <class T, int DP> static __device__ __forceinline__ u32x4 ld_row(const T* s, int row, int c, int h) {
+// A tile of ROWS rows in LDS.
+template <class T, int DP, int ROWS> struct LdsTile {
     using G = Geo<T, DP>;
-    return *(const u32x4*)(s + row * G::LD + c * G::CH + h * G::EL);
-}
-
-// left operand, transposed: column d0 + lane % 32 of the tile at the contraction rows of chunk c (order: see pack), counted from row0
-template <class T, int DP> static __device__ __forceinline__ u32x4 ld_t(const T* s, int row0, int c, int d0, int lane) {
-    using G = Geo<T, DP>;
-    const int h = lane >> 5;
-    if constexpr (sizeof(T) == 4) {
-        const float* p = (const float*)s + (row0 + 8 * c + 4 * h) * G::LD + d0 + (lane & 31);
-        f32x4 y = {p[0], p[G::LD], p[2 * G::LD], p[3 * G::LD]};
-        return __builtin_bit_cast(u32x4, y);
-    } else {
-        // ds_read_b64_tr_b16: the 16 lanes of a group name the 16 eight-byte pieces of a 4 (rows) x 16 (columns) block; lane i receives column i
-        const int i = lane & 15;
-        const T* p = s + (row0 + 16 * c + 4 * h + (i >> 2)) * G::LD + d0 + (lane & 16) + (i & 3) * 4;
-        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * G::LD));
-        struct { s16x4 a, b; } both = {lo, hi};
-        return __builtin_bit_cast(u32x4, both);
+    using E = typename Term<T>::E;
+    E* s;
+    // left operand, row-major: chunk c of row `row`
+    __device__ __forceinline__ Frag<T> row(int row, int c, int h) const {
+        Frag<T> f;
+#pragma unroll
+        for (int i = 0; i < Term<T>::N; ++i) f.p[i] = *(const u32x4*)(s + i * G::plane(ROWS) + row * G::LD + c * 16 + h * 8);
+        return f;
     }
-}
+    // left operand, transposed: column d0 + lane % 32 at the contraction rows of chunk c (order: see pack), counted from row0.
+    // ds_read_b64_tr_b16: the 16 lanes of a group name the 16 eight-byte pieces of a 4 (rows) x 16 (columns) block; lane i receives column i.
+    __device__ __forceinline__ Frag<T> column(int row0, int c, int d0, int lane) const {
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const int h = lane >> 5, i = lane & 15;
+        E* p = s + (row0 + 16 * c + 4 * h + (i >> 2)) * G::LD + d0 + (lane & 16) + (i & 3) * 4;
+        Frag<T> f;
+#pragma unroll
+        for (int n = 0; n < Term<T>::N; ++n) {
+            struct { s16x4 a, b; } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + n * G::plane(ROWS))),
+                                           __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + n * G::plane(ROWS) + 8 * G::LD))};
+            f.p[n] = __builtin_bit_cast(u32x4, both);
+        }
+        return f;
+    }
+};
 
-// ---- tiles of rows between global memory, registers and LDS -----------------------------------------------------------------
+// ---- tiles of rows from global memory by way of registers -------------------------------------------------------------------
 // Rows of any stride (multiples of 16 bytes); what lies outside [0, nrows) x [0, D) reads as zero, so that whatever a masked place
 // holds (infinities, NaN) never meets a product.
 template <class T, int DP, int ROWS> struct RowTile {
     using G = Geo<T, DP>;
+    using E = typename Term<T>::E;
     static constexpr int N = (ROWS * G::CPR + CA_THREADS - 1) / CA_THREADS;
     u32x4 r[N];
     __device__ __forceinline__ void load(const T* base, long stride, int nrows, int D, int tid) {
@@ -133,11 +186,24 @@ template <class T, int DP, int ROWS> struct RowTile {
             }
         }
     }
-    __device__ __forceinline__ void store(T* s, int tid) const {
+    __device__ __forceinline__ void store(const LdsTile<T, DP, ROWS>& t, int tid) const {
 #pragma unroll
         for (int v = 0; v < N; ++v) {
             const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
-            if (ROWS * G::CPR % CA_THREADS == 0 || row < ROWS) *(u32x4*)(s + row * G::LD + ch * G::EL) = r[v];
+            if (ROWS * G::CPR % CA_THREADS != 0 && row >= ROWS) continue;
+            E* to = t.s + row * G::LD + ch * G::EL;
+            if constexpr (Term<T>::N == 3) {
+                using V4 = __attribute__((ext_vector_type(4))) E;
+                f32x4 x = __builtin_bit_cast(f32x4, r[v]);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                    const V4 y = __builtin_convertvector(x, V4);
+                    *(V4*)(to + n * G::plane(ROWS)) = y;
+                    if (n < 2) x -= __builtin_convertvector(y, f32x4);
+                }
+            } else {
+                *(u32x4*)to = r[v];
+            }
         }
     }
 };
@@ -157,7 +223,7 @@ static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
 }
 
 // Workgroups per CU that the registers are budgeted for (as many waves per SIMD): two where a workgroup's tiles fit 256 registers, else one.
-template <class T, int DP> constexpr int FWD_PER_CU = sizeof(T) == 2 || DP <= 32 ? 2 : 1;
+template <class T, int DP> constexpr int FWD_PER_CU = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 template <class T, int DP> constexpr int BWD_PER_CU = (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1;
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
@@ -167,10 +233,9 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
     constexpr int RED = NWK > 1 ? 4 * (DP + 2) * 32 * 4 : 0;                    // bytes of the joining of waves
-    constexpr int TILE = 2 * BK * G::LD * (int)sizeof(T);
+    constexpr int TILE = 2 * G::bytes(BK);
     __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
-    T* sK = (T*)smem;
-    T* sV = sK + BK * G::LD;
+    const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
     const int w = xcd_order(blockIdx.x, gridDim.x);
@@ -184,13 +249,9 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
 
     const int row = tile * 32 * NWQ + wq * 32 + (lane & 31), u = row / share, g = row - u * share;
     const bool live = row < R;
-    u32x4 qf[G::NCH];
+    Frag<T> qf[G::NCH];
 #pragma unroll
-    for (int c = 0; c < G::NCH; ++c) {
-        qf[c] = u32x4{0, 0, 0, 0};
-        const int d = c * G::CH + h * G::EL;
-        if (live && d < a.D) qf[c] = *(const u32x4*)(q + u * a.q_u + g * a.q_h + d);
-    }
+    for (int c = 0; c < G::NCH; ++c) qf[c] = live ? frag_at(q + u * a.q_u + g * a.q_h, c * 16 + h * 8, a.D) : no_frag<T>();
     f32x16 acc[G::NDT];
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
@@ -216,7 +277,7 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
         for (int t = 0; t < KT; ++t) {
             s[t] = f32x16{0};
 #pragma unroll
-            for (int c = 0; c < G::NCH; ++c) s[t] = Mma<T>::run(s[t], ld_row<T, DP>(sK, (wk * KT + t) * 32 + (lane & 31), c, h), qf[c]);
+            for (int c = 0; c < G::NCH; ++c) s[t] = mma<T>(s[t], sK.row((wk * KT + t) * 32 + (lane & 31), c, h), qf[c]);
         }
         if (k0 + (wk * KT + KT) * 32 > end) {
 #pragma unroll
@@ -251,10 +312,10 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
                 l += s[t][r];
             }
 #pragma unroll
-            for (int c = 0; c < G::PCH; ++c) {
-                const u32x4 p = pack<T>(s[t], c);
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> p = pack<T>(s[t], c);
 #pragma unroll
-                for (int i = 0; i < G::NDT; ++i) acc[i] = Mma<T>::run(acc[i], ld_t<T, DP>(sV, (wk * KT + t) * 32, c, i * 32, lane), p);
+                for (int i = 0; i < G::NDT; ++i) acc[i] = mma<T>(acc[i], sV.column((wk * KT + t) * 32, c, i * 32, lane), p);
             }
         }
     }
@@ -332,16 +393,16 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnAr
     const int d = (int)(i - row * per) * 4;
     const float* ml = a.part + (long)a.nsplit * n * a.D;
     float mj = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) mj = fmaxf(mj, ml[(s * n + row) * 2]);
     f32x4 acc = {0, 0, 0, 0};
     float l = 0.f;
+#pragma unroll 4
     for (int s = 0; s < a.nsplit; ++s) {
-        const float m = ml[(s * n + row) * 2], ls = ml[(s * n + row) * 2 + 1];
-        if (ls == 0.f) continue;                       // (an empty range)
-        const float f = __builtin_amdgcn_exp2f((m - mj) * a.c);
-        const f32x4 x = *(const f32x4*)(a.part + (s * n + row) * a.D + d);
-        l += f * ls;
-        acc += f * x;
+        const float m = ml[(s * n + row) * 2];
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mj) * a.c);      // (an empty range: zeros)
+        l += f * ml[(s * n + row) * 2 + 1];
+        acc += f * *(const f32x4*)(a.part + (s * n + row) * a.D + d);
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     using V4 = __attribute__((ext_vector_type(4))) T;
@@ -357,10 +418,9 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
     constexpr int RED = NWK > 1 ? 4 * DP * 32 * 4 : 0;
-    constexpr int TILE = 2 * BK * G::LD * (int)sizeof(T);
+    constexpr int TILE = 2 * G::bytes(BK);
     __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
-    T* sK = (T*)smem;
-    T* sV = sK + BK * G::LD;
+    const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
     const int w = xcd_order(blockIdx.x, gridDim.x);
@@ -378,19 +438,18 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
         tk.load(k, a.k_t, end, a.D, tid);
         tv.load(v, a.v_t, end, a.D, tid);
     }
-    u32x4 qf[G::NCH], dof[G::NCH];
+    Frag<T> qf[G::NCH], dof[G::NCH];
     float delta = 0.f;
 #pragma unroll
     for (int c = 0; c < G::NCH; ++c) {
-        qf[c] = dof[c] = u32x4{0, 0, 0, 0};
-        const int d = c * G::CH + h * G::EL;
-        if (live && d < a.D) {
-            using VE = __attribute__((ext_vector_type(G::EL))) T;
-            qf[c] = *(const u32x4*)(q + u * a.q_u + g * a.q_h + d);
-            dof[c] = *(const u32x4*)((const T*)a.dout + out_row * a.D + d);
-            const VE x = *(const VE*)((const T*)a.o + out_row * a.D + d), y = __builtin_bit_cast(VE, dof[c]);
+        qf[c] = dof[c] = no_frag<T>();
+        const int d = c * 16 + h * 8;
+        if (live) {
+            const f32x8 x = values_at((const T*)a.o + out_row * a.D, d, a.D), y = values_at((const T*)a.dout + out_row * a.D, d, a.D);
 #pragma unroll
-            for (int e = 0; e < G::EL; ++e) delta = fmaf((float)x[e], (float)y[e], delta);
+            for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);
+            qf[c] = frag_at(q + u * a.q_u + g * a.q_h, d, a.D);
+            dof[c] = frag_of<T>(y);
         }
     }
     delta += other_half(delta);
@@ -416,8 +475,8 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
             f32x16 s = f32x16{0}, dp = f32x16{0};
 #pragma unroll
             for (int c = 0; c < G::NCH; ++c) {
-                s = Mma<T>::run(s, ld_row<T, DP>(sK, r0 + (lane & 31), c, h), qf[c]);
-                dp = Mma<T>::run(dp, ld_row<T, DP>(sV, r0 + (lane & 31), c, h), dof[c]);
+                s = mma<T>(s, sK.row(r0 + (lane & 31), c, h), qf[c]);
+                dp = mma<T>(dp, sV.row(r0 + (lane & 31), c, h), dof[c]);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -425,10 +484,10 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
                 s[r] = k0 + r0 + 8 * (r >> 2) + 4 * h + (r & 3) < end ? p * (dp[r] - delta) : 0.f;
             }
 #pragma unroll
-            for (int c = 0; c < G::PCH; ++c) {
-                const u32x4 ds = pack<T>(s, c);
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> ds = pack<T>(s, c);
 #pragma unroll
-                for (int i = 0; i < G::NDT; ++i) acc[i] = Mma<T>::run(acc[i], ld_t<T, DP>(sK, r0, c, i * 32, lane), ds);
+                for (int i = 0; i < G::NDT; ++i) acc[i] = mma<T>(acc[i], sK.column(r0, c, i * 32, lane), ds);
             }
         }
     }
@@ -471,11 +530,10 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
     constexpr int BR = 32 * RT * NWR;
     constexpr float P_BACK = P_SHIFT<T> == 0.f ? 1.f : 1.f / 16384.f;
     constexpr int RED = NWR > 1 ? 4 * DP * 32 * 4 : 0;
-    constexpr int TILE = 2 * BR * G::LD * (int)sizeof(T) + 2 * BR * 4;
+    constexpr int TILE = 2 * G::bytes(BR) + 2 * BR * 4;
     __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
-    T* sQ = (T*)smem;
-    T* sO = sQ + BR * G::LD;
-    float* sL = (float*)(sO + BR * G::LD);
+    const LdsTile<T, DP, BR> sQ{(typename Term<T>::E*)smem}, sO{(typename Term<T>::E*)(smem + G::bytes(BR))};
+    float* sL = (float*)(smem + 2 * G::bytes(BR));
     float* sD = sL + BR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
@@ -505,14 +563,13 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
         tq.load_rows(q, a.q_u, a.q_h, 0, R, share, a.D, tid);
         to.load_rows(dout, (long)a.H * a.D, a.D, 0, R, share, a.D, tid);
         stats(0);
-        u32x4 kf[G::NCH], vf[G::NCH];
+        Frag<T> kf[G::NCH], vf[G::NCH];
 #pragma unroll
         for (int c = 0; c < G::NCH; ++c) {
-            kf[c] = vf[c] = u32x4{0, 0, 0, 0};
-            const int d = c * G::CH + h * G::EL;
-            if (key < len && d < a.D) {
-                kf[c] = *(const u32x4*)((const T*)a.k + b * a.k_b + kvh * a.k_h + (long)key * a.k_t + d);
-                vf[c] = *(const u32x4*)((const T*)a.v + b * a.v_b + kvh * a.v_h + (long)key * a.v_t + d);
+            kf[c] = vf[c] = no_frag<T>();
+            if (key < len) {
+                kf[c] = frag_at((const T*)a.k + b * a.k_b + kvh * a.k_h + (long)key * a.k_t, c * 16 + h * 8, a.D);
+                vf[c] = frag_at((const T*)a.v + b * a.v_b + kvh * a.v_h + (long)key * a.v_t, c * 16 + h * 8, a.D);
             }
         }
         for (int r0 = 0; r0 < R; r0 += BR) {
@@ -533,8 +590,8 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
                 f32x16 s = f32x16{0}, dp = f32x16{0};
 #pragma unroll
                 for (int c = 0; c < G::NCH; ++c) {
-                    s = Mma<T>::run(s, ld_row<T, DP>(sQ, x0 + (lane & 31), c, h), kf[c]);
-                    dp = Mma<T>::run(dp, ld_row<T, DP>(sO, x0 + (lane & 31), c, h), vf[c]);
+                    s = mma<T>(s, sQ.row(x0 + (lane & 31), c, h), kf[c]);
+                    dp = mma<T>(dp, sO.row(x0 + (lane & 31), c, h), vf[c]);
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -547,12 +604,12 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < G::PCH; ++c) {
-                    const u32x4 p = pack<T>(s, c), ds = pack<T>(dp, c);
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> p = pack<T>(s, c), ds = pack<T>(dp, c);
 #pragma unroll
                     for (int i = 0; i < G::NDT; ++i) {
-                        dv[i] = Mma<T>::run(dv[i], ld_t<T, DP>(sO, x0, c, i * 32, lane), p);
-                        dk[i] = Mma<T>::run(dk[i], ld_t<T, DP>(sQ, x0, c, i * 32, lane), ds);
+                        dv[i] = mma<T>(dv[i], sO.column(x0, c, i * 32, lane), p);
+                        dk[i] = mma<T>(dk[i], sQ.column(x0, c, i * 32, lane), ds);
                     }
                 }
             }
@@ -606,6 +663,14 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
 // ---- launch rules -----------------------------------------------------------------------------------------------------------
 constexpr int CA_CUS = 256;
 
+// Forward: 128 rows per workgroup read (and split into terms) every key once per 128 rows instead of once per 32: taken where that gives every CU a
+// workgroup, or where the keys are long enough to be cut into ranges that do (4 x 333 rows of 8 heads over 2999 fp32 keys: 139 us at 32 rows,
+// 66 us at 128 rows in five ranges).
+bool fwd_wide(int B, int U, int T, int H, int Hkv) {
+    const long R = (long)U * (H / Hkv), n = (long)B * Hkv * ((R + 127) / 128);
+    return R > 64 && (n >= CA_CUS || T >= 1024);
+}
+
 template <class K> int launch(K kernel, long grid, const CrossAttnArgs& a, hipStream_t stream) {
     if (grid > 0x7fffffffL) return fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", grid);
     if (grid == 0) return LAS_OK;
@@ -614,23 +679,30 @@ template <class K> int launch(K kernel, long grid, const CrossAttnArgs& a, hipSt
     return LAS_OK;
 }
 
+// Two shapes of a workgroup's four waves: 128 rows (keys) with every wave at all of a key (row) tile, where that gives every CU a workgroup; else
+// fewer rows, the waves side by side over the key (row) tile and joined at the end: 32 rows, or 64 where the tile of four waves (32 keys each, three
+// planes of fp32 terms) would not fit LDS.
+template <class T, int DP> constexpr int NARROW = sizeof(T) == 4 && DP > 64 ? 2 : 1;
+template <class T, int DP> constexpr int DEEP = sizeof(T) == 4 && DP > 64 ? 1 : 2;      // tiles of 32 per pass of the wide shape
+
 template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
-    const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv, n = bh * a.nsplit;
+    constexpr int NQ = NARROW<T, DP>;
+    const long R = (long)a.U * (a.H / a.Hkv), n = (long)a.B * a.Hkv * a.nsplit;
     int rc;
-    // rows per workgroup: 128 where that still gives every CU a workgroup, else 32 with the waves side by side over the keys
-    if (R > 32 && n * ((R + 127) / 128) >= CA_CUS) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, 2>, n * ((R + 127) / 128), a, stream);
-    else rc = launch(cross_attn_fwd_kernel<T, DP, 1, 4, 1>, n * ((R + 31) / 32), a, stream);
+    if (fwd_wide(a.B, a.U, a.T, a.H, a.Hkv)) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, DEEP<T, DP>>, n * ((R + 127) / 128), a, stream);
+    else rc = launch(cross_attn_fwd_kernel<T, DP, NQ, 4 / NQ, 1>, n * ((R + 32 * NQ - 1) / (32 * NQ)), a, stream);
     if (rc != LAS_OK || a.nsplit == 1) return rc;
     const long items = (long)a.B * a.U * a.H * (a.D / 4);
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
 template <class T, int DP> int bwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
+    constexpr int NQ = NARROW<T, DP>;
     const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
-    if (bh * ((R + 127) / 128) >= CA_CUS) LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 4, 1, 2>, bh * ((R + 127) / 128), a, stream));
-    else LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 1, 4, 1>, bh * ((R + 31) / 32), a, stream));
-    if (bh * ((a.T + 127) / 128) >= CA_CUS) return launch(cross_attn_dkv_kernel<T, DP, 4, 1, 2>, bh * ((a.T + 127) / 128), a, stream);
-    return launch(cross_attn_dkv_kernel<T, DP, 1, 4, 1>, bh * ((a.T + 31) / 32), a, stream);
+    if (bh * ((R + 127) / 128) >= CA_CUS) LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 4, 1, DEEP<T, DP>>, bh * ((R + 127) / 128), a, stream));
+    else LAS_TRY(launch(cross_attn_dq_kernel<T, DP, NQ, 4 / NQ, 1>, bh * ((R + 32 * NQ - 1) / (32 * NQ)), a, stream));
+    if (bh * ((a.T + 127) / 128) >= CA_CUS) return launch(cross_attn_dkv_kernel<T, DP, 4, 1, DEEP<T, DP>>, bh * ((a.T + 127) / 128), a, stream);
+    return launch(cross_attn_dkv_kernel<T, DP, NQ, 4 / NQ, 1>, bh * ((a.T + 32 * NQ - 1) / (32 * NQ)), a, stream);
 }
 
 template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stream) {
@@ -647,8 +719,8 @@ template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stre
 // Key ranges of a forward call: as many as fill the chip twice over where the rows alone do not, none shorter than 512 keys (a range costs its
 // workgroups a partial result in fp32 and the joining launch).
 int cross_attn_splits(int B, int U, int T, int H, int Hkv) {
-    const long R = (long)U * (H / Hkv), wgs = (long)B * Hkv * ((R + 31) / 32);
-    const long want = 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / 512;
+    const long R = (long)U * (H / Hkv), per = fwd_wide(B, U, T, H, Hkv) ? 128 : 32, wgs = (long)B * Hkv * ((R + per - 1) / per);
+    const long want = wgs >= CA_CUS ? 1 : 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / 512;
     return (int)(want < 2 || most < 2 ? 1 : (want < most ? want : most));
 }
 

@@ -2,6 +2,7 @@
 utterance, heads of keys and values, utterances of different lengths, fp32 / bf16 / fp16 (``las_cross_attention_fwd`` / ``_bwd``)."""
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -15,11 +16,15 @@ def _rows(t, per16):
     sb, st, sh, sd = t.stride()
     if sd == 1 and not (sb | st | sh) % per16 and not t.data_ptr() & 15:
         return t
-    t = t.contiguous()
+    return _aligned(t.contiguous())
+
+
+def _aligned(t):
     return t if not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _check(query, key, value, key_lengths):
+def _refuse(query, key, value):
+    """The first thing that is wrong with the operands."""
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not t.is_cuda:
             raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
@@ -29,67 +34,79 @@ def _check(query, key, value, key_lengths):
             raise RuntimeError("cross_attention: query, key and value must share one type and device")
     if query.dtype not in DTYPES:
         raise RuntimeError(f"cross_attention computes in fp32, bf16 or fp16; got {query.dtype}")
-    B, U, H, D = query.shape
+    B, _U, H, D = query.shape
     if key.shape != value.shape or key.shape[0] != B or key.shape[3] != D:
         raise RuntimeError(f"cross_attention: query {tuple(query.shape)}, key {tuple(key.shape)}, value {tuple(value.shape)} do not go together")
     Hkv = key.shape[2]
     if H < 1 or Hkv < 1 or H % Hkv:
         raise RuntimeError(f"cross_attention: {H} query heads do not share {Hkv} key heads evenly")
-    per16 = 4 if query.dtype == torch.float32 else 8
-    if not 0 < D <= 128 or D % per16:
-        raise RuntimeError(f"cross_attention: the head size must be a multiple of {per16} and at most 128, got {D}")
+    raise RuntimeError(f"cross_attention: the head size must be a multiple of {4 if query.dtype == torch.float32 else 8} and at most 128, got {D}")
+
+
+def _lengths(key_lengths, B, T, device):
+    if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"cross_attention: key_lengths must be ({B},) int32 or int64, got {tuple(key_lengths.shape)} {key_lengths.dtype}")
+    if key_lengths.device != device:
+        raise RuntimeError("cross_attention: key_lengths must be on the device of the query")
+    if key_lengths.dtype != torch.int32:
+        key_lengths = key_lengths.clamp(0, T).to(torch.int32)
+    return key_lengths.contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_floats(B, U, T, H, Hkv, D):
+    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D), 0)
+
+
+def _forward(query, key, value, key_lengths, scale, want_lse):
+    dtype = query.dtype
+    qs, ks = query.shape, key.shape
+    code = DTYPES.get(dtype)
+    if (code is None or len(qs) != 4 or len(ks) != 4 or ks != value.shape or not query.is_cuda or key.dtype != dtype or value.dtype != dtype
+            or key.device != query.device or value.device != query.device):
+        _refuse(query, key, value)
+    B, U, H, D = qs
+    T, Hkv = ks[1], ks[2]
+    per16 = 4 if code == 0 else 8
+    if ks[0] != B or ks[3] != D or Hkv < 1 or H < 1 or H % Hkv or not 0 < D <= 128 or D % per16:
+        _refuse(query, key, value)
+    device = query.device
     if key_lengths is not None:
-        if key_lengths.shape != (B,) or key_lengths.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError(f"cross_attention: key_lengths must be ({B},) int32 or int64, got {tuple(key_lengths.shape)} {key_lengths.dtype}")
-        if key_lengths.device != query.device:
-            raise RuntimeError("cross_attention: key_lengths must be on the device of the query")
-        if key_lengths.dtype != torch.int32:
-            key_lengths = key_lengths.clamp(0, key.shape[1]).to(torch.int32)
-        key_lengths = key_lengths.contiguous()
-    return per16, key_lengths
-
-
-def _forward(query, key, value, key_lengths, scale, per16, want_lse):
+        key_lengths = _lengths(key_lengths, B, T, device)
     q, k, v = _rows(query, per16), _rows(key, per16), _rows(value, per16)
-    B, U, H, D = q.shape
-    T, Hkv = k.shape[1], k.shape[2]
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    d = CrossAttentionDesc(B, U, T, H, Hkv, D, DTYPES[q.dtype], scale, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
-    out = torch.empty(B, U, H, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, U, H, device=q.device, dtype=torch.float32) if want_lse else None
-    L = lib()
-    n = L.las_cross_attention_workspace_floats(d, 0)
-    work = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-    _cabi.call_on(q.device, L.las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    d = CrossAttentionDesc(B, U, T, H, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    out = torch.empty(qs, device=device, dtype=dtype)
+    lse = torch.empty((B, U, H), device=device, dtype=torch.float32) if want_lse else None
+    n = _workspace_floats(B, U, T, H, Hkv, D)
+    work = torch.empty(n, device=device, dtype=torch.float32) if n else None
+    _cabi.call_on(device, lib().las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                   None if work is None else work.data_ptr())
-    return d, q, k, v, out, lse
+    return d, q, k, v, key_lengths, out, lse
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, key_lengths, scale, per16):
-        d, q, k, v, out, lse = _forward(query, key, value, key_lengths, scale, per16, True)
-        ctx.save_for_backward(q, k, v, key_lengths, out, lse)
+    def forward(ctx, query, key, value, key_lengths, scale):
+        d, *saved = _forward(query, key, value, key_lengths, scale, True)
+        ctx.save_for_backward(*saved)
         ctx.desc = d
-        return out
+        return saved[4]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_cabi.differentiable_once
     def backward(ctx, dout):
         q, k, v, key_lengths, out, lse = ctx.saved_tensors
-        dout = dout.contiguous()
-        if dout.data_ptr() & 15:
-            dout = dout.clone(memory_format=torch.contiguous_format)
-        dev = q.device
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        dv = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        delta = torch.empty(lse.shape, device=dev, dtype=torch.float32)
-        _cabi.call_on(dev, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        dout = _aligned(dout.contiguous())
+        device = q.device
+        dq = torch.empty_like(out)
+        dk = torch.empty(k.shape, device=device, dtype=k.dtype)
+        dv = torch.empty_like(dk)
+        delta = torch.empty_like(lse)
+        _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                       dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr())
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None
 
 
 def cross_attention(query, key, value, key_lengths=None, scale=None):
@@ -101,8 +118,6 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
     any gives zeros.  ``scale`` defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once) in query, key and value.
     Scores, softmax and sums are fp32 whatever the type.  U = 1 is one decode step: the key range is split over the GPU where the batch
     alone does not fill it.  Rows that are not contiguous or not 16-byte aligned are copied first."""
-    per16, key_lengths = _check(query, key, value, key_lengths)
-    scale = 1.0 / math.sqrt(query.shape[3]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
-        return _CrossAttentionFn.apply(query, key, value, key_lengths, scale, per16)
-    return _forward(query, key, value, key_lengths, scale, per16, False)[4]
+        return _CrossAttentionFn.apply(query, key, value, key_lengths, scale)
+    return _forward(query, key, value, key_lengths, scale, False)[5]

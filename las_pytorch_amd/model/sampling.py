@@ -2,6 +2,8 @@
 ``Speller.forward_step`` themselves; ``Speller.sample`` is such a loop."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _cabi
@@ -19,6 +21,11 @@ def _limit(name, value, B, device, whole=False):
         value = value.clamp(0, 2 ** 31 - 1).to(torch.int32)
     value = (value if whole else value.to(torch.float32)).contiguous()
     return 0, value.data_ptr(), value
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(B, V):
+    return lib().las_sample_workspace_bytes(B, V)
 
 
 def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -57,9 +64,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     uniforms = uniforms.contiguous()
     tokens = torch.empty(B, device=dev, dtype=torch.int64)
     logprob = torch.empty(B, device=dev, dtype=torch.float32)
-    L = lib()
-    n = L.las_sample_workspace_bytes(B, V)
+    n = _workspace_bytes(B, V)
     work = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-    _cabi.call_on(dev, L.las_sample_tokens, logits.data_ptr(), logits.stride(0), DTYPES[logits.dtype], B, V, uniforms.data_ptr(), t, min(k, 2 ** 31 - 1), p, m,
+    _cabi.call_on(dev, lib().las_sample_tokens, logits.data_ptr(), logits.stride(0), DTYPES[logits.dtype], B, V, uniforms.data_ptr(), t, min(k, 2 ** 31 - 1), p, m,
                   tr, kr, pr, mr, tokens.data_ptr(), logprob.data_ptr(), None if work is None else work.data_ptr())
     return tokens, logprob

@@ -18,6 +18,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from .. import _cabi
+
 CLIP_NORM = 1.0     # the reference hard-codes clip_grad_norm_(..., 1) (solver/solver.py:96; the YAML's max_norm is unused)
 
 
@@ -182,11 +184,9 @@ class _DistillationLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_cabi.differentiable_once
     def backward(ctx, upstream):
-        from .. import _cabi
         logits, index, teacher, lengths = ctx.saved_tensors
-        upstream = upstream.to(torch.float32).contiguous()
         grad, ctx.grad = ctx.grad, None
         if grad is not None:
             _cabi.call_on(grad.device, _cabi.lib().las_scale_unless_one, grad.data_ptr(), grad.numel(), _cabi.DTYPES[grad.dtype], upstream.data_ptr())
@@ -197,18 +197,18 @@ class _DistillationLoss(torch.autograd.Function):
 
 
 def _distill(logits, index, teacher, lengths, temperature, want_loss, grad, upstream):
-    from .. import _cabi
     B, U, V = logits.shape
-    K = index.shape[2]
     dev = logits.device
-    out = torch.empty(1 + B * U, device=dev, dtype=torch.float32) if want_loss else None      # the loss, then the rows' scratch
-    at = out.data_ptr() if want_loss else None
-    gs = (0, 0) if grad is None else (grad.stride(1), grad.stride(0))
-    _cabi.call_on(dev, _cabi.lib().las_distill_loss, logits.data_ptr(), logits.stride(1), logits.stride(0), _cabi.DTYPES[logits.dtype],
-                  index.data_ptr(), int(index.dtype == torch.int64), teacher.data_ptr(), _cabi.DTYPES[teacher.dtype],
-                  None if lengths is None else lengths.data_ptr(), B, U, V, K, temperature, at, None if grad is None else grad.data_ptr(),
-                  gs[0], gs[1], None if upstream is None else upstream.data_ptr(), at + 4 if want_loss else None)
-    return out[0] if want_loss else None
+    loss = torch.empty((), device=dev, dtype=torch.float32) if want_loss else None
+    rows = torch.empty(B * U, device=dev, dtype=torch.float32) if want_loss else None
+    gb, gu = (0, 0) if grad is None else grad.stride()[:2]
+    zb, zu, _ = logits.stride()
+    _cabi.call_on(dev, _cabi.lib().las_distill_loss, logits.data_ptr(), zu, zb, _cabi.DTYPES[logits.dtype],
+                  index.data_ptr(), index.dtype == torch.int64, teacher.data_ptr(), _cabi.DTYPES[teacher.dtype],
+                  None if lengths is None else lengths.data_ptr(), B, U, V, index.shape[2], temperature,
+                  loss.data_ptr() if want_loss else None, None if grad is None else grad.data_ptr(),
+                  gu, gb, None if upstream is None else upstream.data_ptr(), rows.data_ptr() if want_loss else None)
+    return loss
 
 
 def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=1.0, lengths=None):
@@ -223,7 +223,6 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     counts with both entries; a row without entries, like an utterance without steps, adds nothing.  ``lengths`` (B,) int32 / int64 on the
     device, clamped to [0, U]; None: every step counts.  Returns a scalar fp32 tensor, differentiable (once) in ``pred_y``; its gradient has
     the type of ``pred_y`` and is zero on steps that do not count."""
-    from .. import _cabi
     if not pred_y.is_cuda:
         raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
     if pred_y.dim() != 3 or pred_y.dtype not in _cabi.DTYPES:
