@@ -161,15 +161,19 @@ template <class T, int DP, int ROWS> struct LdsTile {
 // ---- tiles of rows from global memory by way of registers -------------------------------------------------------------------
 // Rows of any stride (multiples of 16 bytes); what lies outside [0, nrows) x [0, D) reads as zero, so that whatever a masked place
 // holds (infinities, NaN) never meets a product.
-template <class T, int DP, int ROWS> struct RowTile {
+constexpr int pow2_from(int n) { int p = 1; while (p < n) p *= 2; return p; }
+
+// P: pieces that a row takes of the threads (its CPR, or the next power of two where the threads of a row have to add something up)
+template <class T, int DP, int ROWS, int P = Geo<T, DP>::CPR> struct RowTile {
     using G = Geo<T, DP>;
     using E = typename Term<T>::E;
-    static constexpr int N = (ROWS * G::CPR + CA_THREADS - 1) / CA_THREADS;
+    static constexpr int N = (ROWS * P + CA_THREADS - 1) / CA_THREADS;
+    static_assert(P == G::CPR || ROWS * P % 64 == 0, "a row's threads lie in one wave");
     u32x4 r[N];
     __device__ __forceinline__ void load(const T* base, long stride, int nrows, int D, int tid) {
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
+            const int i = tid + v * CA_THREADS, row = i / P, ch = i % P;
             r[v] = u32x4{0, 0, 0, 0};
             if (row < nrows && row < ROWS && ch * G::EL < D) r[v] = *(const u32x4*)(base + row * stride + ch * G::EL);
         }
@@ -178,7 +182,7 @@ template <class T, int DP, int ROWS> struct RowTile {
     __device__ __forceinline__ void load_rows(const T* base, long su, long sg, int row0, int nrows, int share, int D, int tid) {
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
+            const int i = tid + v * CA_THREADS, row = i / P, ch = i % P;
             r[v] = u32x4{0, 0, 0, 0};
             if (row0 + row < nrows && row < ROWS && ch * G::EL < D) {
                 const int u = share == 1 ? row0 + row : (row0 + row) / share, g = row0 + row - u * share;
@@ -189,8 +193,8 @@ template <class T, int DP, int ROWS> struct RowTile {
     __device__ __forceinline__ void store(const LdsTile<T, DP, ROWS>& t, int tid) const {
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            const int i = tid + v * CA_THREADS, row = i / G::CPR, ch = i % G::CPR;
-            if (ROWS * G::CPR % CA_THREADS != 0 && row >= ROWS) continue;
+            const int i = tid + v * CA_THREADS, row = i / P, ch = i % P;
+            if ((ROWS * P % CA_THREADS != 0 && row >= ROWS) || (P != G::CPR && ch >= G::CPR)) continue;
             E* to = t.s + row * G::LD + ch * G::EL;
             if constexpr (Term<T>::N == 3) {
                 using V4 = __attribute__((ext_vector_type(4))) E;
@@ -204,6 +208,21 @@ template <class T, int DP, int ROWS> struct RowTile {
             } else {
                 *(u32x4*)to = r[v];
             }
+        }
+    }
+    // to[row] = f times the inner product of this tile's rows with another's, in fp32 (the sum's order is that of a tree over the row's threads)
+    __device__ __forceinline__ void products(const RowTile& other, float f, float* to, int tid) const {
+        using V = __attribute__((ext_vector_type(G::EL))) T;
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int i = tid + v * CA_THREADS, row = i / P;
+            const V x = __builtin_bit_cast(V, r[v]), y = __builtin_bit_cast(V, other.r[v]);
+            float d = 0.f;
+#pragma unroll
+            for (int e = 0; e < G::EL; ++e) d = fmaf((float)x[e], (float)y[e], d);
+#pragma unroll
+            for (int o = P / 2; o > 0; o >>= 1) d += __shfl_xor(d, o);
+            if (i % P == 0 && row < ROWS) to[row] = d * f;
         }
     }
 };
@@ -411,19 +430,20 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnAr
     if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
 }
 
-// ---- backward: dq (and D_i) -------------------------------------------------------------------------------------------------
+// ---- backward: dq -----------------------------------------------------------------------------------------------------------
 // The forward's shape: one row per lane; q and do stay in registers, every key tile is read once per row tile.
+template <class T, int DP, int NWQ, int NWK, int KT> constexpr int DQ_BYTES() {
+    const int tile = 2 * Geo<T, DP>::bytes(32 * KT * NWK), red = NWK > 1 ? 4 * DP * 32 * 4 : 0;
+    return tile > red ? tile : red;
+}
 template <class T, int DP, int NWQ, int NWK, int KT>
-__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq_kernel(CrossAttnArgs a) {
+static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int block, int blocks, char* smem) {
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
-    constexpr int RED = NWK > 1 ? 4 * DP * 32 * 4 : 0;
-    constexpr int TILE = 2 * G::bytes(BK);
-    __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
     const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
-    const int w = xcd_order(blockIdx.x, gridDim.x);
+    const int w = xcd_order(block, blocks);
     const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
     const int end = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
@@ -453,7 +473,6 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
         }
     }
     delta += other_half(delta);
-    if (live && wk == 0 && h == 0) a.delta[out_row] = delta;
     const float lse = live ? a.lse[out_row] : INFINITY;
     f32x16 acc[G::NDT];
 #pragma unroll
@@ -524,25 +543,28 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dq
 
 // ---- backward: dk, dv -------------------------------------------------------------------------------------------------------
 // One key per lane (k and v in registers), row tiles of q and do through LDS; NWK waves side by side over keys, NWR over rows.
+// D_i is formed here once more, by the threads that bring in a row of do (and for that alone the same row of the output): the two halves of the
+// backward then need nothing of each other and run in one launch, the one filling the other's last round.
+template <class T, int DP, int NWK, int NWR, int RT> constexpr int DKV_BYTES() {
+    const int tile = 2 * Geo<T, DP>::bytes(32 * RT * NWR) + 2 * 32 * RT * NWR * 4, red = NWR > 1 ? 4 * DP * 32 * 4 : 0;
+    return tile > red ? tile : red;
+}
 template <class T, int DP, int NWK, int NWR, int RT>
-__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dkv_kernel(CrossAttnArgs a) {
+static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, int block, int blocks, char* smem) {
     using G = Geo<T, DP>;
     constexpr int BR = 32 * RT * NWR;
     constexpr float P_BACK = P_SHIFT<T> == 0.f ? 1.f : 1.f / 16384.f;
-    constexpr int RED = NWR > 1 ? 4 * DP * 32 * 4 : 0;
-    constexpr int TILE = 2 * G::bytes(BR) + 2 * BR * 4;
-    __shared__ __attribute__((aligned(16))) char smem[TILE > RED ? TILE : RED];
     const LdsTile<T, DP, BR> sQ{(typename Term<T>::E*)smem}, sO{(typename Term<T>::E*)(smem + G::bytes(BR))};
     float* sL = (float*)(smem + 2 * G::bytes(BR));
     float* sD = sL + BR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
-    const int w = xcd_order(blockIdx.x, gridDim.x);
+    const int w = xcd_order(block, blocks);
     const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
     const int len = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const long row_base = (long)b * a.U * a.H + kvh * share;
-    const T* dout = (const T*)a.dout + row_base * a.D;
+    const T *dout = (const T*)a.dout + row_base * a.D, *out = (const T*)a.o + row_base * a.D;
     const int key = tile * 32 * NWK + wk * 32 + (lane & 31);
     const bool any = tile * 32 * NWK < len;             // (workgroup-uniform)
 
@@ -550,19 +572,20 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i) dk[i] = dv[i] = f32x16{0};
     if (any) {
-        RowTile<T, DP, BR> tq, to;
-        float rl = INFINITY, rd = 0.f;
-        auto stats = [&](int r0) {
-            rl = INFINITY; rd = 0.f;                    // rows behind the last: p = exp2(s - inf) = 0
+        RowTile<T, DP, BR> tq;
+        RowTile<T, DP, BR, pow2_from(G::CPR)> to, ty;
+        float rl = INFINITY;
+        auto fetch = [&](int r0) {
+            tq.load_rows(q, a.q_u, a.q_h, r0, R, share, a.D, tid);
+            to.load_rows(dout, (long)a.H * a.D, a.D, r0, R, share, a.D, tid);
+            ty.load_rows(out, (long)a.H * a.D, a.D, r0, R, share, a.D, tid);
+            rl = INFINITY;                              // rows behind the last: p = exp2(s - inf) = 0
             if (tid < BR && r0 + tid < R) {
                 const int u = (r0 + tid) / share, g = r0 + tid - u * share;
                 rl = a.lse[row_base + (long)u * a.H + g] - P_SHIFT<T>;
-                rd = a.delta[row_base + (long)u * a.H + g] * P_BACK;
             }
         };
-        tq.load_rows(q, a.q_u, a.q_h, 0, R, share, a.D, tid);
-        to.load_rows(dout, (long)a.H * a.D, a.D, 0, R, share, a.D, tid);
-        stats(0);
+        fetch(0);
         Frag<T> kf[G::NCH], vf[G::NCH];
 #pragma unroll
         for (int c = 0; c < G::NCH; ++c) {
@@ -576,13 +599,10 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
             __syncthreads();
             tq.store(sQ, tid);
             to.store(sO, tid);
-            if (tid < BR) { sL[tid] = rl; sD[tid] = rd; }
+            to.products(ty, P_BACK, sD, tid);
+            if (tid < BR) sL[tid] = rl;
             __syncthreads();
-            if (r0 + BR < R) {
-                tq.load_rows(q, a.q_u, a.q_h, r0 + BR, R, share, a.D, tid);
-                to.load_rows(dout, (long)a.H * a.D, a.D, r0 + BR, R, share, a.D, tid);
-                stats(r0 + BR);
-            }
+            if (r0 + BR < R) fetch(r0 + BR);
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int x0 = (wr * RT + t) * 32;
@@ -660,6 +680,15 @@ __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_dk
         }
 }
 
+// One launch: the key side's workgroups first (they are the longer ones), then the row side's.
+template <class T, int DP, int NW, int DEPTH>
+__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int keys_blocks) {
+    constexpr int A = DKV_BYTES<T, DP, NW, 4 / NW, DEPTH>(), B = DQ_BYTES<T, DP, NW, 4 / NW, DEPTH>();
+    __shared__ __attribute__((aligned(16))) char smem[A > B ? A : B];
+    if ((int)blockIdx.x < keys_blocks) cross_attn_dkv<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x, keys_blocks, smem);
+    else cross_attn_dq<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x - keys_blocks, gridDim.x - keys_blocks, smem);
+}
+
 // ---- launch rules -----------------------------------------------------------------------------------------------------------
 constexpr int CA_CUS = 256;
 
@@ -696,13 +725,17 @@ template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
+// Backward: both sides wide where that makes two workgroups per CU, else both narrow.
 template <class T, int DP> int bwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
     constexpr int NQ = NARROW<T, DP>;
     const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
-    if (bh * ((R + 127) / 128) >= CA_CUS) LAS_TRY(launch(cross_attn_dq_kernel<T, DP, 4, 1, DEEP<T, DP>>, bh * ((R + 127) / 128), a, stream));
-    else LAS_TRY(launch(cross_attn_dq_kernel<T, DP, NQ, 4 / NQ, 1>, bh * ((R + 32 * NQ - 1) / (32 * NQ)), a, stream));
-    if (bh * ((a.T + 127) / 128) >= CA_CUS) return launch(cross_attn_dkv_kernel<T, DP, 4, 1, DEEP<T, DP>>, bh * ((a.T + 127) / 128), a, stream);
-    return launch(cross_attn_dkv_kernel<T, DP, NQ, 4 / NQ, 1>, bh * ((a.T + 32 * NQ - 1) / (32 * NQ)), a, stream);
+    const bool wide = bh * ((R + 127) / 128 + (a.T + 127) / 128) >= 2 * CA_CUS;
+    const long per = wide ? 128 : 32 * NQ, rows = bh * ((R + per - 1) / per), keys = bh * ((a.T + per - 1) / per);
+    if (rows + keys > 0x7fffffffL) return fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", rows + keys);
+    if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
+    else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, NQ, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
+    LAS_LAUNCH_CHECK();
+    return LAS_OK;
 }
 
 template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stream) {

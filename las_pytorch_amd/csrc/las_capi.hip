@@ -1484,10 +1484,9 @@ CrossAttnArgs cross_attention_args(const las_cross_attention_desc* d, const void
 
 }  // namespace
 
-size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d, int backward) {
+size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d) {
     if (!d || d->B <= 0 || d->U <= 0 || d->T < 0 || d->H <= 0 || d->Hkv <= 0 || d->D <= 0) return 0;
     const size_t rows = (size_t)d->B * d->U * d->H;
-    if (backward) return rows;
     const int n = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv);
     return n > 1 ? rows * n * (d->D + 2) : 0;
 }
@@ -1506,16 +1505,15 @@ int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, co
 }
 
 int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
-                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* workspace,
-                            void* stream) {
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* stream) {
     LAS_TRY(cross_attention_check(d, q, k, v));
     if (d->B == 0) return LAS_OK;
     const bool rows = d->U > 0, keys = d->T > 0;
-    LAS_REQUIRE(!rows || (out && lse && dout && dq && workspace), "cross attention backward pointers");
+    LAS_REQUIRE(!rows || (out && lse && dout && dq), "cross attention backward pointers");
     LAS_REQUIRE(!keys || (dk && dv), "cross attention gradients");
     LAS_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "cross attention tensors: 16-byte aligned");
     CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
-    a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.delta = workspace;
+    a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
     return cross_attn(a, d->dtype, true, (hipStream_t)stream);
 }
 

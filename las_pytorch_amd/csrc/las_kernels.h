@@ -359,11 +359,11 @@ int collate_pad(const float* packed, const long long* foff, const long long* pla
 // ---- cross_attn.hip --------------------------------------------------------------------
 // Attention of U decoder states per utterance over T encoder states, H query heads on Hkv key / value heads, head size D (<= 128).
 // Strides in elements; q: batch, step, head; k / v: batch, frame, head (rows of D contiguous, 16-byte aligned).  o, dout, dq (B,U,H,D), dk, dv
-// (B,T,Hkv,D) contiguous; lse, delta (B,U,H) fp32 (lse in units of log 2).  part: nsplit (B U H) (D + 2) floats when nsplit > 1.
+// (B,T,Hkv,D) contiguous; lse (B,U,H) fp32, in units of log 2.  part: nsplit (B U H) (D + 2) floats when nsplit > 1.
 struct CrossAttnArgs {
     const void *q, *k, *v, *dout;
     void *o, *dq, *dk, *dv;
-    float *lse, *delta, *part;
+    float *lse, *part;
     const int* lens;               // valid frames per utterance (clamped to [0, T]); NULL: all
     long q_b, q_u, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
     int B, U, T, H, Hkv, D, nsplit;

@@ -55,7 +55,7 @@ def _lengths(key_lengths, B, T, device):
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_floats(B, U, T, H, Hkv, D):
-    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D), 0)
+    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D))
 
 
 def _forward(query, key, value, key_lengths, scale, want_lse):
@@ -102,10 +102,9 @@ class _CrossAttentionFn(torch.autograd.Function):
         dq = torch.empty_like(out)
         dk = torch.empty(k.shape, device=device, dtype=k.dtype)
         dv = torch.empty_like(dk)
-        delta = torch.empty_like(lse)
         _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr())
+                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None
 
 

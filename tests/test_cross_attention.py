@@ -296,7 +296,7 @@ def test_c_entry_refuses_before_it_launches():
                    dict(U=1 << 30), dict(T=1 << 30)):
         d = _cabi.CrossAttentionDesc(**{**good, **change})
         assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, 4096, None, None, None) == 1, change
-        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, 4096, None) == 1, change
+        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, None) == 1, change
         assert b"cross attention" in L.las_last_error()
     d = _cabi.CrossAttentionDesc(**good)
     for at in range(3):
@@ -306,10 +306,10 @@ def test_c_entry_refuses_before_it_launches():
         ptrs[at] = 4100
         assert L.las_cross_attention_fwd(d, *ptrs, None, 4096, None, None, None) == 1
     assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, None, None, None, None) == 1
-    assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, None, 4096, 4096, 4096, 4096, 4096, None) == 1
+    assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, None, 4096, 4096, 4096, 4096, None) == 1
     assert L.las_cross_attention_fwd(None, 4096, 4096, 4096, None, 4096, None, None, None) == 1
-    assert L.las_cross_attention_workspace_floats(d, 1) == 2
-    assert L.las_cross_attention_workspace_floats(_cabi.CrossAttentionDesc(**{**good, "T": 4096}), 0) > 0
+    assert L.las_cross_attention_workspace_floats(d) == 0
+    assert L.las_cross_attention_workspace_floats(_cabi.CrossAttentionDesc(**{**good, "T": 4096})) > 0
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         cross_attention(*(torch.zeros(1, 2, 2, 32) for _ in range(3)))
     assert "cross_attention" in las_pytorch_amd.__all__
