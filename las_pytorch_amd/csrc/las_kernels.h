@@ -399,7 +399,7 @@ struct SampleArgs {
     long z_b;
     int B, V, top_k;
 };
-constexpr int SM_SLICES = 64;      // most slices of a row
+constexpr int SM_SLICES = 64, SM_MOST = 1 << 20;      // most slices of a row, longest row that is cut into them
 int sample_slices(int B, int V);
 size_t sample_workspace_bytes(int B, int V);      // 0: none
 int sample(const SampleArgs& a, int dtype, void* workspace, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16

@@ -76,6 +76,12 @@ struct Weigher {
         return y < (float)(SM_BINS - 1) ? (int)y : SM_BINS - 1;
     }
 };
+// x lies in one of the bins up to `bin` (the same comparison that Weigher::bin makes)
+struct Near {
+    float zmax, af, most;
+    __device__ __forceinline__ Near(const Weigher& w, int bin) : zmax(w.zmax), af(w.af), most(bin < SM_BINS - 1 ? (float)(bin + 1) : INFINITY) {}
+    __device__ __forceinline__ bool operator()(float x) const { return x == zmax || (zmax - x) * af < most; }
+};
 static_assert(SM_TABLE == 256, "Weigher::fixed takes the low eight bits");
 
 struct Limits {
@@ -112,8 +118,19 @@ static __device__ __forceinline__ Weigher weigher(const double* table, float zma
     return w;
 }
 
+struct Powers {
+    double v[SM_TABLE];
+    constexpr Powers() : v() {
+        for (int j = 0; j < SM_TABLE; ++j) {      // the series of exp(j / 256 ln 2), smallest term first
+            double x = 1.0;
+            for (int n = 24; n > 0; --n) x = 1.0 + x * (j * (0.6931471805599453 / SM_TABLE)) / n;
+            v[j] = x;
+        }
+    }
+};
+__device__ const Powers POWERS;
 static __device__ __forceinline__ void fill_table(double* table, int tid, int nt) {
-    for (int i = tid; i < SM_TABLE; i += nt) table[i] = exp2((double)i / SM_TABLE);
+    for (int i = tid; i < SM_TABLE; i += nt) table[i] = POWERS.v[i];
 }
 
 static __device__ __forceinline__ void answer(const SampleArgs& a, int row, int token, float logp) {
@@ -137,9 +154,9 @@ static __device__ __forceinline__ u64 wave_scan(u64 x) {             // inclusiv
 // falling order over the wave
 static __device__ __forceinline__ u64 wave_sort(u64 x) {
     const int lane = threadIdx.x & 63;
-#pragma unroll
+#pragma unroll 1
     for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
+#pragma unroll 1
         for (int o = size >> 1; o > 0; o >>= 1) {
             const u64 y = __shfl_xor(x, o);
             const bool want_large = ((lane & o) == 0) == ((lane & size) == 0);
@@ -274,19 +291,87 @@ template <int NT, class Each> static __device__ __forceinline__ u64 search(u64 t
     return found;
 }
 
-// f(logit, index) for this thread's share of [lo, hi) of a row, sixteen bytes at a time
-template <int NT, class T, class F> static __device__ __forceinline__ void each_logit(const T* z, int lo, int hi, F f) {
-    constexpr int EL = 16 / (int)sizeof(T);
+// f(logit as it is, index) for this thread's share of [lo, hi) of a row: sixteen bytes at a time, four loads in flight
+template <int NT, class T, class F> static __device__ __forceinline__ void each_raw(const T* z, int lo, int hi, F f) {
+    constexpr int EL = 16 / (int)sizeof(T), AHEAD = 4;
     typedef T V __attribute__((ext_vector_type(EL), aligned(sizeof(T))));
-    for (int i = lo + (int)threadIdx.x * EL; i < hi; i += NT * EL) {
-        if (i + EL <= hi) {
-            const V x = *(const V*)(z + i);
+    for (int i0 = lo + (int)threadIdx.x * EL; i0 < hi; i0 += AHEAD * NT * EL) {
+        V x[AHEAD];
 #pragma unroll
-            for (int e = 0; e < EL; ++e) f(clean((T)x[e]), i + e);
-        } else {
-            for (int e = i; e < hi; ++e) f(logit_at(z, e), e);
+        for (int n = 0; n < AHEAD; ++n)
+            if (i0 + n * NT * EL + EL <= hi) x[n] = *(const V*)(z + i0 + n * NT * EL);
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            const int i = i0 + n * NT * EL;
+            if (i + EL <= hi) {
+#pragma unroll
+                for (int e = 0; e < EL; ++e) f((float)x[n][e], i + e);
+            } else {
+                for (int e = i; e < hi; ++e) f((float)z[e], e);
+            }
         }
     }
+}
+// f(logit, index) for this thread's share, one at a time with the next on its way: for bodies of many instructions (a draw is over in the time that
+// a hundred cache lines of instructions take to arrive, so unrolling them costs more than it hides)
+template <int NT, class T, class F> static __device__ __forceinline__ void each_logit(const T* z, int lo, int hi, F f) {
+    int i = lo + (int)threadIdx.x;
+    float next = i < hi ? logit_at(z, i) : 0.f;
+#pragma unroll 1
+    for (; i < hi; i += NT) {
+        const float x = next;
+        next = i + NT < hi ? logit_at(z, i + NT) : 0.f;
+        f(x, i);
+    }
+}
+// found(logit, index) for the few logits of this thread's share (each_raw's) that near(logit) holds for
+template <int NT, class T, class Near, class Found> static __device__ __forceinline__ void each_near(const T* z, int lo, int hi, Near near, Found found) {
+    constexpr int EL = 16 / (int)sizeof(T), AHEAD = 32 / EL;
+    typedef T V __attribute__((ext_vector_type(EL), aligned(sizeof(T))));
+    for (int i0 = lo + (int)threadIdx.x * EL; i0 < hi; i0 += AHEAD * NT * EL) {
+        V x[AHEAD];
+        unsigned hits = 0;
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n)
+            if (i0 + n * NT * EL + EL <= hi) x[n] = *(const V*)(z + i0 + n * NT * EL);
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            const int i = i0 + n * NT * EL;
+            if (i + EL <= hi) {
+#pragma unroll
+                for (int e = 0; e < EL; ++e) hits |= (near((float)x[n][e]) ? 1u : 0u) << (n * EL + e);
+            } else if (i < hi) {
+                for (int e = 0; e < hi - i; ++e) hits |= 1u << (n * EL + e);      // (the row's end: looked at one by one below)
+            }
+        }
+        while (hits) {
+            const int bit = __ffs((int)hits) - 1, i = i0 + bit / EL * NT * EL + bit % EL;
+            hits &= hits - 1;
+            const float v = logit_at(z, i);
+            if (near(v)) found(v, i);
+        }
+    }
+}
+
+// draw_listed for lists that are too long to be sorted
+template <int NT>
+static __device__ __attribute__((noinline)) void search_listed(SampleArgs a, int row, Limits lim, Weigher w, int n, u64 head, Shared& s) {
+    const int tid = threadIdx.x;
+    auto each = [&](auto f) { for (int i = tid; i < n; i += NT) f(s.place[i], w.fixed(logit_of(s.place[i]))); };
+    u64 cut = 0, m = 0;
+    if (lim.by_count(a.V)) cut = search<NT>((u64)min(lim.top_k, (long)n), 64, [&](auto f) { each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
+    if (lim.by_mass()) {
+        each([&](u64 p, u64 x) { if (p >= cut) m += x; });
+        const u64 total = block_sum<NT>(m, s);
+        cut = search<NT>(head ? head : lim.head(total), 64, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut) f(p, x); }); }, s);
+    }
+    const u64 least = lim.least(w.unit);
+    m = 0;
+    each([&](u64 p, u64 x) { if (p >= cut && x >= least) m += x; });
+    const u64 total = block_sum<NT>(m, s);
+    const u64 at = search<NT>(lim.goal(total), 32, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut && x >= least) f((u64)(unsigned)p, x); }); }, s);
+    const int token = (int)~(unsigned)at;
+    each([&](u64 p, u64 x) { if (index_of(p) == token) answer(a, row, token, share(x, total)); });
 }
 
 // Every candidate that can be kept is in s.place[0 .. n): draw.  head: see wave_draw.
@@ -313,21 +398,7 @@ template <int NT> static __device__ void draw_listed(const SampleArgs& a, int ro
         if (incl - x < goal && goal <= incl) answer(a, row, (int)~(unsigned)(p >> 32), share(x, total));
         return;
     }
-    auto each = [&](auto f) { for (int i = tid; i < n; i += NT) f(s.place[i], w.fixed(logit_of(s.place[i]))); };
-    u64 cut = 0, m = 0;
-    if (lim.by_count(a.V)) cut = search<NT>((u64)min(lim.top_k, (long)n), 64, [&](auto f) { each([&](u64 p, u64) { f(p, (u64)1); }); }, s);
-    if (lim.by_mass()) {
-        each([&](u64 p, u64 x) { if (p >= cut) m += x; });
-        const u64 total = block_sum<NT>(m, s);
-        cut = search<NT>(head ? head : lim.head(total), 64, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut) f(p, x); }); }, s);
-    }
-    const u64 least = lim.least(w.unit);
-    m = 0;
-    each([&](u64 p, u64 x) { if (p >= cut && x >= least) m += x; });
-    const u64 total = block_sum<NT>(m, s);
-    const u64 at = search<NT>(lim.goal(total), 32, [&](auto f) { each([&](u64 p, u64 x) { if (p >= cut && x >= least) f((u64)(unsigned)p, x); }); }, s);
-    const int token = (int)~(unsigned)at;
-    each([&](u64 p, u64 x) { if (index_of(p) == token) answer(a, row, token, share(x, total)); });
+    search_listed<NT>(a, row, lim, w, n, head, s);
 }
 
 // The cut in a list of the candidates of one bin: the one at which the running sum (of masses, or of candidates) reaches target.
@@ -391,7 +462,7 @@ template <int NT, class T> static __device__ __forceinline__ u64 cut_in_row(cons
     }, s);
 }
 
-template <class T, int NT> static __device__ void row_draw(const SampleArgs& a, int row, const T* z, const Limits& lim, const Weigher& w, Shared& s) {
+template <class T, int NT> static __device__ __attribute__((noinline)) void row_draw(SampleArgs a, int row, const T* z, Limits lim, Weigher w, Shared& s) {
     const int tid = threadIdx.x, V = a.V;
     u64 cut = 0;                                  // kept: place >= cut
 
@@ -463,20 +534,56 @@ template <class T, int NT> static __device__ void row_draw(const SampleArgs& a, 
     draw_range<NT>(a, row, z, w, cut, least, 0, V, lim.goal(total), total, s);
 }
 
+// top_k of a row without a pass that counts: of the maxima that the threads found in their shares of the row, the top_k-th largest has at least top_k
+// candidates not behind it and, the shares being small, hardly more.  A histogram of these NT maxima alone gives its bin; the candidates down to that
+// bin are the list.  False (nothing done) where the list would be too long or too few threads found a candidate.
+template <class T, int NT>
+static __device__ __forceinline__ bool few_draw(const SampleArgs& a, int row, const T* z, const Limits& lim, const Weigher& w, float mine, Shared& s) {
+    const int tid = threadIdx.x;
+    if (lim.top_k > NT) return false;
+    for (int i = tid; i < SM_BINS; i += NT) s.count[i] = 0;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    if (mine != -INFINITY) atomicAdd(&s.count[w.bin(mine)], 1u);
+    const u64 found = block_sum<NT>(mine != -INFINITY, s);
+    if (found < (u64)lim.top_k) return false;
+    int bin; u64 before;
+    reach<NT>(SM_BINS, (u64)lim.top_k, [&](int i) { return (u64)s.count[i]; }, s, bin, before);
+    if (mine != -INFINITY && w.bin(mine) <= bin) {
+        each_near<NT>(z, 0, a.V, Near(w, bin), [&](float x, int i) {      // its share again
+            if (x == -INFINITY || w.bin(x) > bin) return;
+            const unsigned at = atomicAdd(&s.n, 1u);
+            if (at < SM_CAP) s.place[at] = place_of(x, i);
+        });
+    }
+    __syncthreads();
+    const unsigned n = s.n;
+    if (n > SM_CAP) return false;
+    draw_listed<NT>(a, row, lim, w, (int)n, 0, s);
+    return true;
+}
+
 template <class T, int NT> __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a) {
     __shared__ Shared s;
     const int tid = threadIdx.x, row = blockIdx.x;
     const T* z = (const T*)a.z + row * a.z_b;
     const Limits lim(a, row);
-    u64 best = 0;
-    each_logit<NT>(z, 0, a.V, [&](float x, int i) { best = larger(best, place_of(x, i)); });
-    best = block_max<NT>(best, s);
-    const float zmax = logit_of(best);
+    float mine = -INFINITY;                       // (a NaN loses every comparison)
+    each_raw<NT>(z, 0, a.V, [&](float x, int) { mine = fmaxf(mine, x); });
+    const float zmax = logit_of(block_max<NT>(place_of(mine + 0.f, 0), s));
     if (zmax == -INFINITY) { if (tid == 0) answer(a, row, -1, -INFINITY); return; }        // nothing to draw from
-    if (lim.greedy()) { if (tid == 0) answer(a, row, index_of(best), 0.f); return; }
+    if (lim.greedy()) {
+        u64 best = 0;
+        each_logit<NT>(z, 0, a.V, [&](float x, int i) { best = larger(best, place_of(x, i)); });
+        best = block_max<NT>(best, s);
+        if (tid == 0) answer(a, row, index_of(best), 0.f);
+        return;
+    }
     fill_table(s.table, tid, NT);
     __syncthreads();
-    row_draw<T, NT>(a, row, z, lim, weigher(s.table, zmax, lim.temperature, a.V), s);
+    const Weigher w = weigher(s.table, zmax, lim.temperature, a.V);
+    if (lim.by_count(a.V) && few_draw<T, NT>(a, row, z, lim, w, mine, s)) return;
+    row_draw<T, NT>(a, row, z, lim, w, s);
 }
 
 // rows of at most 64 logits: a wave each
@@ -500,25 +607,27 @@ template <class T> __global__ __launch_bounds__(SW_THREADS) void sample_wave_ker
 }
 
 // ---- the row in slices ------------------------------------------------------------------------------------------------------
-constexpr int SL_THREADS = 512;
+constexpr int SL_THREADS = 512, SM_CHUNK = SL_THREADS, SM_CHUNKS = SM_MOST / SM_CHUNK;
 
 // How a row is drawn once its histogram is known: LISTED every candidate that can be kept goes to the list, CUT only those of the bin of the cut
 // (the bins before it are kept whole), WHOLE everything is kept, ALONE a bin is longer than the list: one workgroup takes the row by itself.
 enum Mode : int { LISTED, CUT, WHOLE, ALONE };
 
+constexpr int SM_GROUP = SM_BINS / 64;
 // workspace of one row
 struct RowSpace {
-    u64 mass[SM_BINS];
-    unsigned count[SM_BINS];
+    u64 mass[SM_BINS], mass_of[64];        // by bin, and by groups of SM_GROUP bins
+    unsigned count[SM_BINS], count_of[64];
     u64 place[SM_CAP];
-    u64 slice_max[SM_SLICES], slice_mass[SM_SLICES];
+    u64 slice_max[SM_SLICES], chunk_mass[SM_CHUNKS];
     u64 target, head;              // of the first slice's verdict: mass to reach within the bin, mass that top_p keeps
     int mode;
     unsigned n;
 };
 
+// slices of whole chunks (the masses are kept by chunk, so that the draw looks into one of them alone)
 static __device__ __forceinline__ void slice_of(int V, int S, int i, int& lo, int& hi) {
-    const int per = ((V + S - 1) / S + 7) & ~7;
+    const int per = ((V + S - 1) / S + SM_CHUNK - 1) / SM_CHUNK * SM_CHUNK;
     lo = min(V, i * per);
     hi = min(V, lo + per);
 }
@@ -528,6 +637,7 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_max_kern
     const int tid = threadIdx.x, row = blockIdx.x / S, slice = blockIdx.x - row * S;
     RowSpace& r = space[row];
     for (int i = slice * SL_THREADS + tid; i < SM_BINS; i += S * SL_THREADS) { r.mass[i] = 0; r.count[i] = 0; }
+    if (slice == 0 && tid < 64) { r.mass_of[tid] = 0; r.count_of[tid] = 0; }
     if (slice == 0 && tid == 0) r.n = 0;
     int lo, hi;
     slice_of(a.V, S, slice, lo, hi);
@@ -543,8 +653,33 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_max_kern
     }
 }
 
-static __device__ __forceinline__ u64 row_max(const RowSpace& r, int S, Shared& s) {
-    return block_max<SL_THREADS>((int)threadIdx.x < S ? r.slice_max[threadIdx.x] : 0, s);
+// (every wave by itself: a barrier costs more than the reads)
+static __device__ __forceinline__ u64 row_max(const RowSpace& r, int S) {
+    const int lane = threadIdx.x & 63;
+    u64 x = lane < S ? r.slice_max[lane] : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = larger(x, __shfl_xor(x, o));
+    return x;
+}
+static_assert(SM_SLICES <= 64, "a lane for each slice");
+
+// The bin in which the running sum (masses, or counts) over the row's bins reaches target, the sums of both before it.  Every wave by itself.
+static __device__ __forceinline__ int reach_bin(const RowSpace& r, bool masses, u64 target, u64& mass_before, u64& count_before) {
+    const int lane = threadIdx.x & 63;
+    u64 m = r.mass_of[lane], c = r.count_of[lane], ms = wave_scan(m), cs = wave_scan(c);
+    u64 hit = __ballot((masses ? ms : cs) >= target);
+    const int group = hit ? __ffsll((long long)hit) - 1 : 63;
+    mass_before = __shfl(ms - m, group);
+    count_before = __shfl(cs - c, group);
+    m = lane < SM_GROUP ? r.mass[group * SM_GROUP + lane] : 0;
+    c = lane < SM_GROUP ? r.count[group * SM_GROUP + lane] : 0;
+    ms = mass_before + wave_scan(m);
+    cs = count_before + wave_scan(c);
+    hit = __ballot((masses ? ms : cs) >= target);
+    const int at = hit ? __ffsll((long long)hit) - 1 : SM_GROUP - 1;
+    mass_before = __shfl(ms - m, at);
+    count_before = __shfl(cs - c, at);
+    return group * SM_GROUP + at;
 }
 
 template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_histogram_kernel(SampleArgs a, RowSpace* space, int S) {
@@ -553,9 +688,9 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_histogra
     RowSpace& r = space[row];
     const Limits lim(a, row);
     const bool masses = !lim.by_count(a.V);      // (with top_k the first cut is one of counts)
-    const float zmax = logit_of(row_max(r, S, s));
+    const float zmax = logit_of(row_max(r, S));
     if (zmax == -INFINITY || lim.greedy() || (!lim.by_count(a.V) && !lim.by_mass())) return;
-    fill_table(s.table, tid, SL_THREADS);
+    if (masses) fill_table(s.table, tid, SL_THREADS);
     for (int i = tid; i < SM_BINS; i += SL_THREADS) { s.mass[i] = 0; s.count[i] = 0; }
     __syncthreads();
     const Weigher w = weigher(s.table, zmax, lim.temperature, a.V);
@@ -568,8 +703,29 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_histogra
         if (masses) atomicAdd(&s.mass[b], w.fixed(x));
     });
     __syncthreads();
+    constexpr int PER = SM_BINS / SL_THREADS;
+    u64 m = 0;
+    unsigned c = 0;
     for (int i = tid; i < SM_BINS; i += SL_THREADS)
         if (s.count[i]) { atomicAdd(&r.count[i], s.count[i]); if (masses) atomicAdd(&r.mass[i], s.mass[i]); }
+    for (int i = tid * PER; i < (tid + 1) * PER; ++i) { c += s.count[i]; m += s.mass[i]; }
+#pragma unroll
+    for (int o = 1; o < SM_GROUP / PER; o <<= 1) { m += __shfl_xor(m, o); c += __shfl_xor(c, o); }
+    if (tid % (SM_GROUP / PER) == 0 && c) {
+        atomicAdd(&r.count_of[tid * PER / SM_GROUP], c);
+        if (masses) atomicAdd(&r.mass_of[tid * PER / SM_GROUP], m);
+    }
+}
+
+// this workgroup's candidates, s.place[0 .. s.n), to the row's list
+template <int NT> static __device__ __forceinline__ void append(RowSpace& r, Shared& s) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const unsigned n = min(s.n, (unsigned)SM_CAP);
+    if (tid == 0) s.out[0] = n ? atomicAdd(&r.n, n) : 0;
+    __syncthreads();
+    const unsigned at = (unsigned)s.out[0];
+    for (unsigned i = tid; i < n && at + i < SM_CAP; i += NT) r.place[at + i] = s.place[i];
 }
 
 template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_slice_kernel(SampleArgs a, RowSpace* space, int S) {
@@ -579,38 +735,31 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_slice_ke
     RowSpace& r = space[row];
     const Limits lim(a, row);
     const T* z = (const T*)a.z + row * a.z_b;
-    const u64 best = row_max(r, S, s);
+    const u64 best = row_max(r, S);
     const float zmax = logit_of(best);
     const bool first = slice == 0 && tid == 0;
     if (zmax == -INFINITY || lim.greedy()) return;
-    fill_table(s.table, tid, NT);
-    __syncthreads();
     const Weigher w = weigher(s.table, zmax, lim.temperature, V);
-    const u64 least = lim.least(w.unit);
 
     // every slice comes to the same verdict
     int mode = WHOLE, bin = SM_BINS;
     u64 target = 0, head = 0;
     if (lim.by_count(V) || lim.by_mass()) {
-        u64 c = 0, m = 0;
-        for (int i = tid; i < SM_BINS; i += NT) { s.count[i] = r.count[i]; s.mass[i] = r.mass[i]; c += s.count[i]; m += s.mass[i]; }
-        const u64 all = block_sum<NT>(c, s), mass = block_sum<NT>(m, s);
-        u64 before;
+        const int lane = tid & 63;
+        const u64 all = wave_sum(r.count_of[lane]), mass = wave_sum(r.mass_of[lane]);
+        u64 ahead, before;
         if (lim.by_count(V)) {
             if ((u64)lim.top_k < all) {
-                reach<NT>(SM_BINS, (u64)lim.top_k, [&](int i) { return (u64)s.count[i]; }, s, bin, before);
-                mode = before + s.count[bin] <= SM_CAP ? LISTED : ALONE;
+                bin = reach_bin(r, false, (u64)lim.top_k, before, ahead);
+                mode = ahead + r.count[bin] <= SM_CAP ? LISTED : ALONE;
             } else {
                 mode = lim.by_mass() ? ALONE : WHOLE;      // (fewer candidates than top_k: no masses were counted)
             }
         } else {
             target = head = lim.head(mass);
-            reach<NT>(SM_BINS, target, [&](int i) { return s.mass[i]; }, s, bin, before);
+            bin = reach_bin(r, true, target, before, ahead);
             target -= before;
-            u64 ahead = 0;
-            for (int i = tid; i < bin; i += NT) ahead += s.count[i];
-            ahead = block_sum<NT>(ahead, s);
-            const unsigned here = s.count[bin];
+            const unsigned here = r.count[bin];
             mode = ahead + here <= NT ? LISTED : here <= SM_CAP ? CUT : ALONE;
         }
     }
@@ -618,67 +767,91 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_slice_ke
     if (mode == ALONE) return;
     int lo, hi;
     slice_of(V, S, slice, lo, hi);
-    u64 m = 0;
-    each_logit<NT>(z, lo, hi, [&](float x, int i) {
-        if (x == -INFINITY) return;
-        const int b = w.bin(x);
-        if (b > bin) return;
-        if (mode == LISTED || b == bin) {
-            const unsigned at = atomicAdd(&r.n, 1u);
-            if (at < SM_CAP) r.place[at] = place_of(x, i);
-        } else {
-            const u64 f = w.fixed(x);
-            if (f >= least) m += f;
+    if (mode == LISTED) {
+        // (to LDS first: one addition to the row's counter per workgroup, not one per candidate)
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        each_near<NT>(z, lo, hi, Near(w, bin), [&](float x, int i) {
+            if (x == -INFINITY || w.bin(x) > bin) return;
+            const unsigned at = atomicAdd(&s.n, 1u);
+            if (at < SM_CAP) s.place[at] = place_of(x, i);
+        });
+        append<NT>(r, s);
+        return;
+    }
+    if (tid == 0) s.n = 0;
+    fill_table(s.table, tid, NT);
+    __syncthreads();
+    const u64 least = lim.least(w.unit);
+    constexpr int EL = SM_CHUNK / 64;             // a wave takes a chunk, a lane eight logits of it
+    for (int c = lo + (tid >> 6) * SM_CHUNK; c < hi; c += NT / 64 * SM_CHUNK) {
+        float v[EL];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+            const int i = c + e * 64 + (tid & 63);
+            v[e] = i < hi ? logit_at(z, i) : -INFINITY;
         }
-    });
-    if (mode == LISTED) return;
-    m = block_sum<NT>(m, s);
-    if (tid == 0) r.slice_mass[slice] = m;
+        u64 m = 0;
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+            const int i = c + e * 64 + (tid & 63), b = v[e] == -INFINITY ? SM_BINS + 1 : w.bin(v[e]);
+            if (b < bin) {
+                const u64 f = w.fixed(v[e]);
+                if (f >= least) m += f;
+            } else if (b == bin && mode == CUT) {
+                const unsigned at = atomicAdd(&s.n, 1u);
+                if (at < SM_CAP) s.place[at] = place_of(v[e], i);
+            }
+        }
+        m = wave_sum(m);
+        if ((tid & 63) == 0) r.chunk_mass[c / SM_CHUNK] = m;
+    }
+    if (mode == CUT) append<NT>(r, s);
 }
 
 template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_draw_kernel(SampleArgs a, const RowSpace* space, int S) {
     constexpr int NT = SL_THREADS;
     __shared__ Shared s;
-    __shared__ u64 masses[SM_SLICES];
     const int tid = threadIdx.x, row = blockIdx.x, V = a.V;
     const RowSpace& r = space[row];
     const Limits lim(a, row);
     const T* z = (const T*)a.z + row * a.z_b;
-    const u64 best = row_max(r, S, s);
+    const int mode = r.mode, n = mode == LISTED || mode == CUT ? min((int)r.n, SM_CAP) : 0;
+    const u64 best = row_max(r, S);
     const float zmax = logit_of(best);
     if (zmax == -INFINITY) { if (tid == 0) answer(a, row, -1, -INFINITY); return; }
     if (lim.greedy()) { if (tid == 0) answer(a, row, index_of(best), 0.f); return; }
     fill_table(s.table, tid, NT);
     const Weigher w = weigher(s.table, zmax, lim.temperature, V);
     const u64 least = lim.least(w.unit);
-    const int mode = r.mode, n = mode == LISTED || mode == CUT ? min((int)r.n, SM_CAP) : 0;
     for (int i = tid; i < n; i += NT) s.place[i] = r.place[i];
-    if (tid < S) masses[tid] = r.slice_mass[tid];
     __syncthreads();
     if (mode == ALONE) return row_draw<T, NT>(a, row, z, lim, w, s);
     if (mode == LISTED) return draw_listed<NT>(a, row, lim, w, n, r.head, s);
-    u64 cut = 0;
-    if (mode == CUT) {
-        cut = cut_in_list<NT>(w, true, r.target, n, s);
-        const int per = ((V + S - 1) / S + 7) & ~7;
-        for (int i = tid; i < n; i += NT) {
-            const u64 p = s.place[i];
-            if (p < cut) continue;
-            const u64 f = w.fixed(logit_of(p));
-            if (f >= least) atomicAdd(&masses[index_of(p) / per], f);
-        }
-        __syncthreads();
+    const u64 cut = mode == CUT ? cut_in_list<NT>(w, true, r.target, n, s) : 0;
+    __syncthreads();
+    const int chunks = (V + SM_CHUNK - 1) / SM_CHUNK;
+    u64 m = 0;
+    for (int i = tid; i < chunks; i += NT) m += s.mass[i] = r.chunk_mass[i];
+    __syncthreads();
+    for (int i = tid; i < n; i += NT) {           // (mode CUT) the bin of the cut, as far as it is kept
+        const u64 p = s.place[i], f = p >= cut ? w.fixed(logit_of(p)) : 0;
+        if (f == 0 || f < least) continue;
+        m += f;
+        atomicAdd(&s.mass[index_of(p) / SM_CHUNK], f);
     }
-    const u64 total = block_sum<NT>(tid < S ? masses[tid] : 0, s), goal = lim.goal(total);
+    const u64 total = block_sum<NT>(m, s), goal = lim.goal(total);
     u64 before;
-    int part, lo, hi;
-    reach<NT>(S, goal, [&](int i) { return masses[i]; }, s, part, before);
-    slice_of(V, S, part, lo, hi);
-    draw_range<NT>(a, row, z, w, cut, least, lo, hi, goal - before, total, s);
+    int part;
+    reach<NT>(chunks, goal, [&](int i) { return s.mass[i]; }, s, part, before);
+    draw_range<NT>(a, row, z, w, cut, least, part * SM_CHUNK, min(V, (part + 1) * SM_CHUNK), goal - before, total, s);
 }
 
+static_assert(SM_CHUNKS <= SM_BINS, "the draw keeps the chunks' masses where the histogram was");
+
 template <class T> int by_size(const SampleArgs& a, void* workspace, hipStream_t stream) {
-    const int S = sample_slices(a.B, a.V);
+    // (top_k from one scalar: a workgroup finds a short list in two reads of the row, 64 rows of 32000: 34 us in slices, 16 us here)
+    const int S = a.top_k > 1 && a.top_k <= 512 && !a.top_k_rows ? 1 : sample_slices(a.B, a.V);
     if (a.V <= 64) {
         hipLaunchKernelGGL(sample_wave_kernel<T>, dim3((unsigned)((a.B + 3) / 4)), dim3(SW_THREADS), 0, stream, a);
     } else if (S > 1) {
@@ -704,6 +877,7 @@ template <class T> int by_size(const SampleArgs& a, void* workspace, hipStream_t
 // Slices of a row: the GPU's 256 CUs twice over shared among the rows, no slice shorter than 4096 logits.  One (a workgroup per row, no workspace) where
 // that leaves no more than one.
 int sample_slices(int B, int V) {
+    if (V > SM_MOST) return 1;
     const int want = B > 0 ? 512 / B : 1, most = V / 4096;
     const int S = want < most ? want : most;
     return S < 2 ? 1 : S > SM_SLICES ? SM_SLICES : S;
