@@ -113,7 +113,21 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         }
     }
     const float c = 1.4426950408889634f / a.tau;
-    float mt = -INFINITY, mz = -INFINITY;
+    // Maximum and sum are taken of each piece as it arrives, relative to the thread's own running maximum: the exponentials of one piece run while the
+    // others are on their way.  (A maximum of -inf stands for an empty sum: exponentials are then taken relative to 0, where they vanish.)
+    auto base = [](float m) { return m == -INFINITY ? 0.f : m; };
+    float mt = -INFINITY, mine = -INFINITY, sz = 0.f, st = 0.f;
+    auto add = [&](V x) {
+        float mx = (float)x[0];
+#pragma unroll
+        for (int e = 1; e < EL; ++e) mx = fmaxf(mx, (float)x[e]);
+        mx = fmaxf(mine, mx);
+        const float b = base(mx);
+        sz *= __builtin_amdgcn_exp2f((mine - b) * c);
+        mine = mx;
+#pragma unroll
+        for (int e = 0; e < EL; ++e) sz += __builtin_amdgcn_exp2f(((float)x[e] - b) * c);
+    };
     for (int k = tid; k < a.K; k += NT) {
         const int v = index_at(a, row * a.K + k);
         const float t = v >= 0 ? teacher_at(a, row * a.K + k) : -INFINITY;
@@ -123,38 +137,17 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     if constexpr (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const V x = held(j);
-#pragma unroll
-            for (int e = 0; e < EL; ++e) mz = fmaxf(mz, (float)x[e]);
+            add(held(j));
+            asm volatile("" : "+v"(sz), "+v"(mine));      // (one piece unpacked at a time: all of them at once would not fit the registers)
         }
     } else {
-        for (int i = tid; i < nvec; i += NT) {
-            const V x = load(i);
-#pragma unroll
-            for (int e = 0; e < EL; ++e) mz = fmaxf(mz, (float)x[e]);
-        }
+        for (int i = tid; i < nvec; i += NT) add(load(i));
     }
+    float mz = mine;
     block2<NT, true>(mt, mz, red);
     if (mt == -INFINITY) { zeros(); return; }    // (no entry at all: nothing to learn from this row)
-    float st = 0.f, sz = 0.f;
-    for (int k = tid; k < a.K; k += NT) {
-        const float e = __builtin_amdgcn_exp2f((sp[k] - mt) * c);
-        st += e;
-    }
-    if constexpr (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const V x = held(j);
-#pragma unroll
-            for (int e = 0; e < EL; ++e) sz += __builtin_amdgcn_exp2f(((float)x[e] - mz) * c);
-        }
-    } else {
-        for (int i = tid; i < nvec; i += NT) {
-            const V x = load(i);
-#pragma unroll
-            for (int e = 0; e < EL; ++e) sz += __builtin_amdgcn_exp2f(((float)x[e] - mz) * c);
-        }
-    }
+    for (int k = tid; k < a.K; k += NT) st += __builtin_amdgcn_exp2f((sp[k] - mt) * c);
+    sz *= __builtin_amdgcn_exp2f((mine - base(mz)) * c);
     block2<NT, false>(st, sz, red);
     const float w = 1.f / ((float)a.B * (float)len);
     const float invt = 1.f / st, invz = 1.f / sz, lt = log2f(st), lz = log2f(sz);
