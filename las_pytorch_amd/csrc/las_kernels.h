@@ -381,7 +381,7 @@ struct DistillArgs {
     const int* lens;               // taught steps per utterance (clamped to [0, U]); NULL: all
     const float* upstream;         // one factor of the gradient on the device; NULL: 1
     long z_b, z_u, dz_b, dz_u;
-    int B, U, V, K, t_dtype, idx64;
+    int B, U, V, K, t_dtype, idx64, stream_out;
     float tau;
 };
 int distill(const DistillArgs& a, int dtype, float* loss, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
