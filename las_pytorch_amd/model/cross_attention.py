@@ -100,7 +100,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         dout = _aligned(dout.contiguous())
         device = q.device
         dq = torch.empty_like(out)
-        dk = torch.empty(k.shape, device=device, dtype=k.dtype)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         dv = torch.empty_like(dk)
         _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),

@@ -667,9 +667,9 @@ class Speller(nn.Module):
         las_model.py:196-198), every step's symbol drawn by ``sample_tokens`` with that function's limits from ``uniforms`` (steps, B) and
         fed back one-hot.  Returns ``(tokens (B, steps) int64, logprob (B, steps) fp32)``; no gradient.  ``temperature`` 0 follows the arg-max,
         like ``decode_mode`` 1."""
-        steps, B = uniforms.shape
-        if listener_feature.shape[0] != B or steps < 1:
-            raise RuntimeError(f"Speller.sample: uniforms must be (steps, {listener_feature.shape[0]}), got {tuple(uniforms.shape)}")
+        B = listener_feature.shape[0]
+        if uniforms.dim() != 2 or uniforms.shape[0] < 1 or uniforms.shape[1] != B:
+            raise RuntimeError(f"Speller.sample: uniforms must be (steps, {B}), got {tuple(uniforms.shape)}")
         with torch.no_grad():
             symbol = torch.zeros(B, dtype=torch.int64, device=listener_feature.device)
             context, state, tokens, logprobs = listener_feature[:, 0], None, [], []

@@ -171,13 +171,16 @@ def label_smoothing_loss_backward_device(pred_y, labels_onehot_int64, label_smoo
 
 class _DistillationLoss(torch.autograd.Function):
     """``las_distill_loss``: the forward leaves the gradient of the loss beside its value (one pass over the logits), the first backward hands
-    it over, multiplied in place where its seed is not one; a further backward of a retained graph forms it again."""
+    it over, multiplied in place where its seed is not one; a further backward of a retained graph forms it again.  In a stream capture the
+    backward forms it always: replayed alone, it would multiply what it has multiplied before."""
 
     @staticmethod
     def forward(ctx, logits, index, teacher, lengths, temperature):
-        grad = torch.empty_like(logits)
-        if grad.stride(2) != 1:
-            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        grad = None
+        if not torch.cuda.is_current_stream_capturing():
+            grad = torch.empty_like(logits)
+            if grad.stride(2) != 1:
+                grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         loss = _distill(logits, index, teacher, lengths, temperature, True, grad, None)
         ctx.save_for_backward(logits, index, teacher, lengths)
         ctx.temperature, ctx.grad = temperature, grad
@@ -187,7 +190,9 @@ class _DistillationLoss(torch.autograd.Function):
     @_cabi.differentiable_once
     def backward(ctx, upstream):
         logits, index, teacher, lengths = ctx.saved_tensors
-        grad, ctx.grad = ctx.grad, None
+        grad = None
+        if not torch.cuda.is_current_stream_capturing():
+            grad, ctx.grad = ctx.grad, None
         if grad is not None:
             _cabi.call_on(grad.device, _cabi.lib().las_scale_unless_one, grad.data_ptr(), grad.numel(), _cabi.DTYPES[grad.dtype], upstream.data_ptr())
         else:

@@ -209,8 +209,37 @@ def test_streams_and_graphs():
         teacher.add_(torch.linspace(0, 1, 20, device="cuda").to(teacher.dtype))
         graph.replay()
         torch.cuda.synchronize()
-        for a, b in zip(step(), held):
-            assert torch.equal(a, b), i
+        loss, grad = step()
+        assert torch.equal(loss, held[0]), i
+        # (the graph's backward has the factor inside, the eager one multiplies a gradient that is rounded to bf16 already: a step of 2^-8 apart)
+        assert ((grad.float() - held[1].float()).abs() <= 2.0 ** -7 * held[1].float().abs()).all(), i
+
+
+@pytest.mark.gpu
+def test_a_backward_captured_alone():
+    """Forward eager, backward in a graph: every replay gives the same gradient (nothing is multiplied twice), and follows its seed.  The forward
+    runs on the stream that captures: autograd runs a backward on its forward's stream, and work on any other stream ends a capture."""
+    z, index, teacher, lengths = _case(torch.float32, 3, 5, 700, 6, seed=10)
+    seed = torch.tensor(2.0, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        zl = z.detach().requires_grad_(True)
+        loss = distillation_loss_device(zl, index, teacher, 2.0, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (held,) = torch.autograd.grad(loss, (zl,), seed, retain_graph=True)
+    for value in (2.0, 2.0, -3.0):
+        seed.fill_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        _, _, want, bound = reference(z, index, teacher, 2.0, lengths, value)
+        assert ((held.double() - want).abs() <= bound).all(), value
+    (eager,) = torch.autograd.grad(loss, (zl,), torch.tensor(1.0, device="cuda"))
+    torch.cuda.synchronize()
+    _, _, want, bound = reference(z, index, teacher, 2.0, lengths)
+    assert ((eager.double() - want).abs() <= bound).all()
 
 
 @pytest.mark.gpu
