@@ -178,16 +178,12 @@ template <class T, int DP, int ROWS, int P = Geo<T, DP>::CPR> struct RowTile {
             if (row < nrows && row < ROWS && ch * G::EL < D) r[v] = *(const u32x4*)(base + row * stride + ch * G::EL);
         }
     }
-    // rows of the (u, g) numbering: row n = u G + g lies at u su + g sg
-    __device__ __forceinline__ void load_rows(const T* base, long su, long sg, int row0, int nrows, int share, int D, int tid) {
+    // the rows that `at` stands at, of those below nrows
+    template <class Walk> __device__ __forceinline__ void load(const T* base, const long (&offset)[N], const Walk& at, int nrows, int D) {
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            const int i = tid + v * CA_THREADS, row = i / P, ch = i % P;
             r[v] = u32x4{0, 0, 0, 0};
-            if (row0 + row < nrows && row < ROWS && ch * G::EL < D) {
-                const int u = share == 1 ? row0 + row : (row0 + row) / share, g = row0 + row - u * share;
-                r[v] = *(const u32x4*)(base + u * su + g * sg + ch * G::EL);
-            }
+            if (at.inside(v, nrows, D)) r[v] = *(const u32x4*)(base + offset[v]);
         }
     }
     __device__ __forceinline__ void store(const LdsTile<T, DP, ROWS>& t, int tid) const {
@@ -223,6 +219,42 @@ template <class T, int DP, int ROWS, int P = Geo<T, DP>::CPR> struct RowTile {
 #pragma unroll
             for (int o = P / 2; o > 0; o >>= 1) d += __shfl_xor(d, o);
             if (i % P == 0 && row < ROWS) to[row] = d * f;
+        }
+    }
+};
+
+// Where this thread's pieces of a tile of ROWS rows lie, row n = u G + g being at u su + g sg of one tensor and of another: divided out once, then carried
+// from tile to tile (a division and two 64-bit products per piece and tile were a third of the key side's vector instructions).
+template <int EL, int ROWS, int P> struct RowWalk {
+    static constexpr int N = (ROWS * P + CA_THREADS - 1) / CA_THREADS;
+    long a[N], b[N], step_a, step_b, wrap_a, wrap_b;
+    int g[N], row0, rest, share, ch, row;
+    __device__ __forceinline__ RowWalk(long su_a, long sg_a, long su_b, long sg_b, int share_, int tid) : row0(0), share(share_), ch(tid % P), row(tid / P) {
+        static_assert(CA_THREADS % P == 0, "a thread keeps its place in the rows");
+        rest = ROWS % share;
+        step_a = ROWS / share * su_a + rest * sg_a; wrap_a = su_a - share * sg_a;
+        step_b = ROWS / share * su_b + rest * sg_b; wrap_b = su_b - share * sg_b;
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            const int n = row + v * (CA_THREADS / P), u = n / share;
+            g[v] = n - u * share;
+            a[v] = u * su_a + g[v] * sg_a + ch * EL;
+            b[v] = u * su_b + g[v] * sg_b + ch * EL;
+        }
+    }
+    __device__ __forceinline__ bool inside(int v, int nrows, int D) const {
+        const int n = row + v * (CA_THREADS / P);
+        return row0 + n < nrows && n < ROWS && ch * EL < D;
+    }
+    __device__ __forceinline__ void next() {
+        row0 += ROWS;
+#pragma unroll
+        for (int v = 0; v < N; ++v) { a[v] += step_a; b[v] += step_b; }
+        if (rest == 0) return;
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            g[v] += rest;
+            if (g[v] >= share) { g[v] -= share; a[v] += wrap_a; b[v] += wrap_b; }
         }
     }
 };
@@ -498,9 +530,11 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
                 dp = mma<T>(dp, sV.row(r0 + (lane & 31), c, h), dof[c]);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
-                s[r] = k0 + r0 + 8 * (r >> 2) + 4 * h + (r & 3) < end ? p * (dp[r] - delta) : 0.f;
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+            if (k0 + r0 + 32 > end) {            // (the keys behind the last: zeros in K, but exp2(-lse) need not be finite)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (k0 + r0 + 8 * (r >> 2) + 4 * h + (r & 3) >= end) s[r] = 0.f;
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -572,20 +606,22 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i) dk[i] = dv[i] = f32x16{0};
     if (any) {
-        RowTile<T, DP, BR> tq;
-        RowTile<T, DP, BR, pow2_from(G::CPR)> to, ty;
+        constexpr int P = pow2_from(G::CPR);
+        RowTile<T, DP, BR, P> tq, to, ty;
+        RowWalk<G::EL, BR, P> at(a.q_u, a.q_h, (long)a.H * a.D, a.D, share, tid);
+        RowWalk<1, BR, 1> ls(0, 0, a.H, 1, share, tid);         // (one row per thread)
         float rl = INFINITY;
-        auto fetch = [&](int r0) {
-            tq.load_rows(q, a.q_u, a.q_h, r0, R, share, a.D, tid);
-            to.load_rows(dout, (long)a.H * a.D, a.D, r0, R, share, a.D, tid);
-            ty.load_rows(out, (long)a.H * a.D, a.D, r0, R, share, a.D, tid);
-            rl = INFINITY;                              // rows behind the last: p = exp2(s - inf) = 0
-            if (tid < BR && r0 + tid < R) {
-                const int u = (r0 + tid) / share, g = r0 + tid - u * share;
-                rl = a.lse[row_base + (long)u * a.H + g] - P_SHIFT<T>;
-            }
+        auto fetch = [&]() {
+            tq.load(q, at.a, at, R, a.D);
+            to.load(dout, at.b, at, R, a.D);
+            ty.load(out, at.b, at, R, a.D);
+            rl = ls.inside(0, R, 1) ? a.lse[row_base + ls.b[0]] - P_SHIFT<T> : INFINITY;      // rows behind the last: p = exp2(s - inf) = 0
+            at.next();
+            ls.next();
         };
-        fetch(0);
+        // (a fp32 tile of wide heads is asked for when it is stored: held through the products it would not fit the registers)
+        constexpr bool EARLY = sizeof(T) == 2 || DP <= 64;
+        if (EARLY) fetch();
         Frag<T> kf[G::NCH], vf[G::NCH];
 #pragma unroll
         for (int c = 0; c < G::NCH; ++c) {
@@ -596,13 +632,14 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
             }
         }
         for (int r0 = 0; r0 < R; r0 += BR) {
+            if (!EARLY) fetch();
             __syncthreads();
             tq.store(sQ, tid);
             to.store(sO, tid);
             to.products(ty, P_BACK, sD, tid);
             if (tid < BR) sL[tid] = rl;
             __syncthreads();
-            if (r0 + BR < R) fetch(r0 + BR);
+            if (EARLY && r0 + BR < R) fetch();
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int x0 = (wr * RT + t) * 32;
