@@ -261,17 +261,32 @@ template <int EL, int ROWS, int P> struct RowWalk {
 
 static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
-// Workgroups of one (utterance, key head) read the same keys: give each XCD (blockIdx % 8 on this device) a contiguous run of work so that
-// they share its L2.  A permutation of [0, n) for any n: correct whatever the placement.  The order runs over utterances first, then heads: an
-// XCD's run then mixes long and short utterances.
-static __device__ __forceinline__ int xcd_order(int b, int n) {
-    const int per = n >> 3, rem = n & 7, x = b & 7, i = b >> 3;
-    return x * per + min(x, rem) + i;
-}
-
 static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
     return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
 }
+
+// Which work a block does.  Workgroups of one (utterance, key head) read the same keys: they go to one XCD (blockIdx % 8 on this device) and share its L2.
+// Where a launch takes more than one round of the GPU (`a.longest_first`), an XCD's workgroups start in falling order of their utterances' lengths and
+// the XCDs take turns in that order, so that the last round fills up with the short ones (16 x 512 over ragged 1500: 259 -> 240 us a step).  A
+// permutation of the work for any placement of blocks.
+struct Work { int i, b, kvh; bool any; };      // i: which of the `per` workgroups of (b, kvh)
+static __device__ __forceinline__ Work work_of(const CrossAttnArgs& a, int block, int per) {
+    const int local = block >> 3, at = (local / per) * 8 + (block & 7), n = a.B * a.Hkv;
+    Work w = {local % per, at / a.Hkv, at % a.Hkv, at < n};
+    if (!a.longest_first || !w.any) return w;
+    // the utterance whose length is the w.b-th largest (equal lengths by index); a lane for each of at most 64
+    const int lane = threadIdx.x & 63, mine = lane < a.B ? length_of(a, lane) : -1;
+    int rank = 0;
+    for (int j = 0; j < a.B; ++j) {
+        const int other = __builtin_amdgcn_readlane(mine, j);
+        rank += other > mine || (other == mine && j < lane) ? 1 : 0;
+    }
+    w.b = __ffsll((long long)__ballot(lane < a.B && rank == w.b)) - 1;
+    return w;
+}
+// blocks of a launch of `per` workgroups for each (utterance, key head)
+static long blocks_of(const CrossAttnArgs& a, long per) { return ((long)a.B * a.Hkv + 7) / 8 * 8 * per; }
+
 
 // Workgroups per CU that the registers are budgeted for (as many waves per SIMD): two where a workgroup's tiles fit 256 registers, else one.
 template <class T, int DP> constexpr int FWD_PER_CU = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
@@ -289,8 +304,9 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
     const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
-    const int w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = w % ntiles, split = (w / ntiles) % a.nsplit, bh = w / (ntiles * a.nsplit), b = bh % a.B, kvh = bh / a.B;
+    const Work w = work_of(a, blockIdx.x, ntiles * a.nsplit);
+    if (!w.any) return;
+    const int tile = w.i % ntiles, split = w.i / ntiles, b = w.b, kvh = w.kvh;
     const int len = length_of(a, b);
     const int per = ((len + a.nsplit - 1) / a.nsplit + 31) & ~31;
     const int begin = min(len, split * per), end = min(len, begin + per);
@@ -469,14 +485,15 @@ template <class T, int DP, int NWQ, int NWK, int KT> constexpr int DQ_BYTES() {
     return tile > red ? tile : red;
 }
 template <class T, int DP, int NWQ, int NWK, int KT>
-static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int block, int blocks, char* smem) {
+static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int block, char* smem) {
     using G = Geo<T, DP>;
     constexpr int BK = 32 * KT * NWK;
     const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
-    const int w = xcd_order(block, blocks);
-    const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
+    const Work w = work_of(a, block, ntiles);
+    if (!w.any) return;
+    const int tile = w.i, b = w.b, kvh = w.kvh;
     const int end = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
@@ -584,7 +601,7 @@ template <class T, int DP, int NWK, int NWR, int RT> constexpr int DKV_BYTES() {
     return tile > red ? tile : red;
 }
 template <class T, int DP, int NWK, int NWR, int RT>
-static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, int block, int blocks, char* smem) {
+static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, int block, char* smem) {
     using G = Geo<T, DP>;
     constexpr int BR = 32 * RT * NWR;
     constexpr float P_BACK = P_SHIFT<T> == 0.f ? 1.f : 1.f / 16384.f;
@@ -593,8 +610,9 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
     float* sD = sL + BR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
-    const int w = xcd_order(block, blocks);
-    const int tile = w % ntiles, bh = w / ntiles, b = bh % a.B, kvh = bh / a.B;
+    const Work w = work_of(a, block, ntiles);
+    if (!w.any) return;
+    const int tile = w.i, b = w.b, kvh = w.kvh;
     const int len = length_of(a, b);
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const long row_base = (long)b * a.U * a.H + kvh * share;
@@ -722,8 +740,8 @@ template <class T, int DP, int NW, int DEPTH>
 __global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int keys_blocks) {
     constexpr int A = DKV_BYTES<T, DP, NW, 4 / NW, DEPTH>(), B = DQ_BYTES<T, DP, NW, 4 / NW, DEPTH>();
     __shared__ __attribute__((aligned(16))) char smem[A > B ? A : B];
-    if ((int)blockIdx.x < keys_blocks) cross_attn_dkv<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x, keys_blocks, smem);
-    else cross_attn_dq<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x - keys_blocks, gridDim.x - keys_blocks, smem);
+    if ((int)blockIdx.x < keys_blocks) cross_attn_dkv<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x, smem);
+    else cross_attn_dq<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x - keys_blocks, smem);
 }
 
 // ---- launch rules -----------------------------------------------------------------------------------------------------------
@@ -737,9 +755,12 @@ bool fwd_wide(int B, int U, int T, int H, int Hkv) {
     return R > 64 && (n >= CA_CUS || T >= 1024);
 }
 
-template <class K> int launch(K kernel, long grid, const CrossAttnArgs& a, hipStream_t stream) {
-    if (grid > 0x7fffffffL) return fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", grid);
+int check_grid(long grid) { return grid <= 0x7fffffffL ? LAS_OK : fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", grid); }
+
+template <class K> int launch(K kernel, long grid, CrossAttnArgs a, hipStream_t stream) {
     if (grid == 0) return LAS_OK;
+    LAS_TRY(check_grid(grid));
+    a.longest_first = a.lens && a.B > 1 && a.B <= 64 && grid > 2 * CA_CUS;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(CA_THREADS), 0, stream, a);
     LAS_LAUNCH_CHECK();
     return LAS_OK;
@@ -753,22 +774,25 @@ template <class T, int DP> constexpr int DEEP = sizeof(T) == 4 && DP > 64 ? 1 : 
 
 template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
     constexpr int NQ = NARROW<T, DP>;
-    const long R = (long)a.U * (a.H / a.Hkv), n = (long)a.B * a.Hkv * a.nsplit;
+    const long R = (long)a.U * (a.H / a.Hkv);
     int rc;
-    if (fwd_wide(a.B, a.U, a.T, a.H, a.Hkv)) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, DEEP<T, DP>>, n * ((R + 127) / 128), a, stream);
-    else rc = launch(cross_attn_fwd_kernel<T, DP, NQ, 4 / NQ, 1>, n * ((R + 32 * NQ - 1) / (32 * NQ)), a, stream);
+    if (fwd_wide(a.B, a.U, a.T, a.H, a.Hkv)) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, DEEP<T, DP>>, blocks_of(a, a.nsplit * ((R + 127) / 128)), a, stream);
+    else rc = launch(cross_attn_fwd_kernel<T, DP, NQ, 4 / NQ, 1>, blocks_of(a, a.nsplit * ((R + 32 * NQ - 1) / (32 * NQ))), a, stream);
     if (rc != LAS_OK || a.nsplit == 1) return rc;
     const long items = (long)a.B * a.U * a.H * (a.D / 4);
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
 // Backward: both sides wide where that makes two workgroups per CU, else both narrow.
-template <class T, int DP> int bwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
+template <class T, int DP> int bwd_dp(const CrossAttnArgs& args, hipStream_t stream) {
     constexpr int NQ = NARROW<T, DP>;
+    CrossAttnArgs a = args;
     const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
     const bool wide = bh * ((R + 127) / 128 + (a.T + 127) / 128) >= 2 * CA_CUS;
-    const long per = wide ? 128 : 32 * NQ, rows = bh * ((R + per - 1) / per), keys = bh * ((a.T + per - 1) / per);
-    if (rows + keys > 0x7fffffffL) return fail(LAS_ERR_UNSUPPORTED, "cross attention: %s%ld workgroups", "", rows + keys);
+    const long per = wide ? 128 : 32 * NQ, rows = blocks_of(a, (R + per - 1) / per), keys = blocks_of(a, (a.T + per - 1) / per);
+    if (rows + keys == 0) return LAS_OK;
+    LAS_TRY(check_grid(rows + keys));
+    a.longest_first = a.lens && a.B > 1 && a.B <= 64 && rows + keys > 2 * CA_CUS;
     if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
     else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, NQ, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
     LAS_LAUNCH_CHECK();

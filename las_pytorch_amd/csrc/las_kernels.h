@@ -366,7 +366,7 @@ struct CrossAttnArgs {
     float *lse, *part;
     const int* lens;               // valid frames per utterance (clamped to [0, T]); NULL: all
     long q_b, q_u, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
-    int B, U, T, H, Hkv, D, nsplit;
+    int B, U, T, H, Hkv, D, nsplit, longest_first;
     float scale, c;                // c = scale log2(e)
 };
 int cross_attn_splits(int B, int U, int T, int H, int Hkv);
