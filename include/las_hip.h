@@ -271,7 +271,7 @@ int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, in
  * Attention of decoder states over an encoder's states of another length.  Beside las_attention_*, which attends one decoder state per
  * utterance with the reference's MLP keys (model/las_model.py:275-318): here U states per utterance, H query heads that share Hkv key /
  * value heads (H a multiple of Hkv; query head h reads head h / (H / Hkv)), and utterances of different lengths.
- *   s[i][j] = scale q_i . k_j over the first key_lengths[b] of T frames,  out_i = sum_j softmax_j(s)[i][j] v_j
+ *   s[i][j] = scale q_i . k_j (scale > 0) over the first key_lengths[b] of T frames,  out_i = sum_j softmax_j(s)[i][j] v_j
  *   An utterance without valid frames gives out = 0 and zero gradients.  What the frames behind key_lengths[b] hold is never read (dk / dv are
  *   written there, as zeros).  key_lengths: int32 (B) on the device, values outside [0, T] count as the nearer end; NULL: every frame is valid.
  *   q (B,U,H,D), k / v (B,T,Hkv,D) of one type (dtype 0 fp32, 1 bf16, 2 fp16), any strides (in elements) with rows of D contiguous; row

@@ -1465,6 +1465,7 @@ int cross_attention_check(const las_cross_attention_desc* d, const void* q, cons
     const int el = d->dtype == 0 ? 4 : 8;
     LAS_REQUIRE(d->D > 0 && d->D <= 128 && d->D % el == 0, "cross attention head size: at most 128 and whole 16-byte pieces");
     LAS_REQUIRE((int64_t)d->U * (d->H / d->Hkv) < (1 << 30) && d->T < (1 << 30), "cross attention lengths");
+    LAS_REQUIRE(d->scale > 0.f && d->scale < 1e38f, "cross attention scale: positive");
     const int64_t strides = d->q_b | d->q_u | d->q_h | d->k_b | d->k_t | d->k_h | d->v_b | d->v_t | d->v_h;
     LAS_REQUIRE(strides % el == 0, "cross attention strides: multiples of 16 bytes");
     LAS_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "cross attention rows: 16-byte aligned");

@@ -129,6 +129,25 @@ def test_values_and_gradients(dtype, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(16, 300, 300, 12, 4, 64), (2, 23, 90, 10, 2, 48), (4, 61, 200, 7, 1, 128), (70, 33, 129, 6, 2, 32)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_groups_that_do_not_divide_a_tile(dtype, shape):
+    """Three, five and seven query heads to a key head, rows that span tiles and heads; more utterances than a wave has lanes."""
+    q, k, v, dout, lengths = _inputs(dtype, *shape, seed=20)
+    _check(q, k, v, dout, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-3, 0.7, 3.0])
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_scales_and_large_scores(dtype, scale):
+    """Scales other than the default: nearly flat rows, and rows whose scores grow from tile to tile by far more than the running maximum may lag."""
+    q, k, v, dout, lengths = _inputs(dtype, 3, 40, 300, 4, 2, 64, seed=21)
+    k = k * torch.linspace(0.1, 1.0, 300, device="cuda").to(dtype)[None, :, None, None]
+    _check(q, k, v, dout, lengths, scale=scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
 def test_what_masked_frames_hold_never_matters(dtype):
     q, k, v, dout, lengths = _inputs(dtype, 5, 9, 70, 4, 2, 64, seed=1)
@@ -275,6 +294,7 @@ def test_refusals():
         (dict(query=q[..., :30], key=k[..., :30], value=v[..., :30]), "head size"),
         (dict(query=torch.zeros(2, 3, 4, 132, device="cuda"), key=torch.zeros(2, 5, 2, 132, device="cuda"), value=torch.zeros(2, 5, 2, 132, device="cuda")),
          "head size"),
+        (dict(scale=0.0), "scale"), (dict(scale=-0.5), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"),
         (dict(key_lengths=lengths.float()), "key_lengths"),
         (dict(key_lengths=lengths[:1]), "key_lengths"),
         (dict(key_lengths=lengths.cpu()), "key_lengths"),
@@ -293,7 +313,7 @@ def test_c_entry_refuses_before_it_launches():
     L = _cabi.lib()
     good = dict(B=1, U=1, T=1, H=2, Hkv=1, D=32, dtype=0, scale=1.0, q_b=64, q_u=64, q_h=32, k_b=32, k_t=32, k_h=32, v_b=32, v_t=32, v_h=32)
     for change in (dict(dtype=3), dict(H=3, Hkv=2), dict(Hkv=0), dict(D=0), dict(D=132), dict(D=30), dict(dtype=1, D=20), dict(B=-1), dict(q_u=65),
-                   dict(U=1 << 30), dict(T=1 << 30)):
+                   dict(U=1 << 30), dict(T=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf)):
         d = _cabi.CrossAttentionDesc(**{**good, **change})
         assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, 4096, None, None, None) == 1, change
         assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, None) == 1, change
