@@ -638,7 +638,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
             ls.next();
         };
         // (a fp32 tile of wide heads is asked for when it is stored: held through the products it would not fit the registers)
-        constexpr bool EARLY = sizeof(T) == 2 || DP <= 64;
+        constexpr bool EARLY = DP <= 64 || (sizeof(T) == 2 && NWR == 1);
         if (EARLY) fetch();
         Frag<T> kf[G::NCH], vf[G::NCH];
 #pragma unroll
@@ -735,13 +735,15 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
         }
 }
 
-// One launch: the key side's workgroups first (they are the longer ones), then the row side's.
+// One launch: the side whose workgroups take longer first (`keys_first`, else the row side's), its `first` blocks before the other's.
 template <class T, int DP, int NW, int DEPTH>
-__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int keys_blocks) {
+__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int first, int keys_first) {
     constexpr int A = DKV_BYTES<T, DP, NW, 4 / NW, DEPTH>(), B = DQ_BYTES<T, DP, NW, 4 / NW, DEPTH>();
     __shared__ __attribute__((aligned(16))) char smem[A > B ? A : B];
-    if ((int)blockIdx.x < keys_blocks) cross_attn_dkv<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x, smem);
-    else cross_attn_dq<T, DP, NW, 4 / NW, DEPTH>(a, blockIdx.x - keys_blocks, smem);
+    const bool second = (int)blockIdx.x >= first;
+    const int block = second ? blockIdx.x - first : blockIdx.x;
+    if (second != (keys_first != 0)) cross_attn_dkv<T, DP, NW, 4 / NW, DEPTH>(a, block, smem);
+    else cross_attn_dq<T, DP, NW, 4 / NW, DEPTH>(a, block, smem);
 }
 
 // ---- launch rules -----------------------------------------------------------------------------------------------------------
@@ -766,10 +768,10 @@ template <class K> int launch(K kernel, long grid, CrossAttnArgs a, hipStream_t 
     return LAS_OK;
 }
 
-// Two shapes of a workgroup's four waves: 128 rows (keys) with every wave at all of a key (row) tile, where that gives every CU a workgroup; else
-// fewer rows, the waves side by side over the key (row) tile and joined at the end: 32 rows, or 64 where the tile of four waves (32 keys each, three
-// planes of fp32 terms) would not fit LDS.
-template <class T, int DP> constexpr int NARROW = sizeof(T) == 4 && DP > 64 ? 2 : 1;
+// Two shapes of a workgroup's four waves: wide, 128 rows (keys) with every wave at all of a key (row) tile; narrow, fewer rows, the waves side by side over
+// the key (row) tile too and joined at the end: 64 rows, in the forward of small 16-bit heads 32.  (32 rows in the backward, or of wide heads, hold
+// tiles of 128 of the other side: one workgroup to a CU, 20 against 12.5 us at 8 x 128 over 375 heads of 64, 70 against 27 at 4 x 400 over 500 heads of 96.)
+template <class T, int DP> constexpr int NARROW = sizeof(T) == 4 || DP > 64 ? 2 : 1;
 template <class T, int DP> constexpr int DEEP = sizeof(T) == 4 && DP > 64 ? 1 : 2;      // tiles of 32 per pass of the wide shape
 
 template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
@@ -783,18 +785,21 @@ template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
-// Backward: both sides wide where that makes two workgroups per CU, else both narrow.
+// Backward: both sides wide where that makes two workgroups per CU, fp32 one (its narrow shape has a CU to itself too: 41 against 56 us at 32 x 128
+// over 100 heads of 128; not where most of 128 rows would be empty), else both narrow.
 template <class T, int DP> int bwd_dp(const CrossAttnArgs& args, hipStream_t stream) {
-    constexpr int NQ = NARROW<T, DP>;
     CrossAttnArgs a = args;
     const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
-    const bool wide = bh * ((R + 127) / 128 + (a.T + 127) / 128) >= 2 * CA_CUS;
-    const long per = wide ? 128 : 32 * NQ, rows = blocks_of(a, (R + per - 1) / per), keys = blocks_of(a, (a.T + per - 1) / per);
+    const long n = bh * ((R + 127) / 128 + (a.T + 127) / 128);
+    const bool wide = n >= 2 * CA_CUS || (sizeof(T) == 4 && R > 64 && n >= CA_CUS);
+    const long per = wide ? 128 : 64, rows = blocks_of(a, (R + per - 1) / per), keys = blocks_of(a, (a.T + per - 1) / per);
     if (rows + keys == 0) return LAS_OK;
     LAS_TRY(check_grid(rows + keys));
     a.longest_first = a.lens && a.B > 1 && a.B <= 64 && rows + keys > 2 * CA_CUS;
-    if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
-    else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, NQ, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, (int)keys);
+    // (a workgroup of the key side goes over the rows in 16 products a tile, one of the row side over the keys in 12)
+    const int keys_first = R * 4 >= (long)a.T * 3, first = (int)(keys_first ? keys : rows);
+    if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
+    else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 2, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
     LAS_LAUNCH_CHECK();
     return LAS_OK;
 }
@@ -810,11 +815,11 @@ template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stre
 
 }  // namespace
 
-// Key ranges of a forward call: as many as fill the chip twice over where the rows alone do not, none shorter than 512 keys (a range costs its
-// workgroups a partial result in fp32 and the joining launch).
-int cross_attn_splits(int B, int U, int T, int H, int Hkv) {
+// Key ranges of a forward call: as many as fill the chip twice over where the rows alone do not, none shorter than 256 keys (512 at 128 rows, 128 of
+// fp32, whose tiles take longer): a range costs its workgroups a partial result in fp32 and the joining launch.
+int cross_attn_splits(int B, int U, int T, int H, int Hkv, int dtype) {
     const long R = (long)U * (H / Hkv), per = fwd_wide(B, U, T, H, Hkv) ? 128 : 32, wgs = (long)B * Hkv * ((R + per - 1) / per);
-    const long want = wgs >= CA_CUS ? 1 : 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / 512;
+    const long want = wgs >= CA_CUS ? 1 : 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / (dtype == 0 ? 128 : per == 128 ? 512 : 256);
     return (int)(want < 2 || most < 2 ? 1 : (want < most ? want : most));
 }
 

@@ -1488,7 +1488,7 @@ CrossAttnArgs cross_attention_args(const las_cross_attention_desc* d, const void
 size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d) {
     if (!d || d->B <= 0 || d->U <= 0 || d->T < 0 || d->H <= 0 || d->Hkv <= 0 || d->D <= 0) return 0;
     const size_t rows = (size_t)d->B * d->U * d->H;
-    const int n = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv);
+    const int n = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv, d->dtype);
     return n > 1 ? rows * n * (d->D + 2) : 0;
 }
 
@@ -1499,7 +1499,7 @@ int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, co
     LAS_REQUIRE(out && ((uintptr_t)out & 15) == 0, "cross attention output");
     CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
     a.o = out; a.lse = lse;
-    a.nsplit = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv);
+    a.nsplit = cross_attn_splits(d->B, d->U, d->T, d->H, d->Hkv, d->dtype);
     LAS_REQUIRE(a.nsplit == 1 || (workspace && ((uintptr_t)workspace & 15) == 0), "cross attention workspace");
     a.part = workspace;
     return cross_attn(a, d->dtype, false, (hipStream_t)stream);

@@ -369,7 +369,7 @@ struct CrossAttnArgs {
     int B, U, T, H, Hkv, D, nsplit, longest_first;
     float scale, c;                // c = scale log2(e)
 };
-int cross_attn_splits(int B, int U, int T, int H, int Hkv);
+int cross_attn_splits(int B, int U, int T, int H, int Hkv, int dtype);
 int cross_attn(const CrossAttnArgs& a, int dtype, bool bwd, hipStream_t stream);      // dtype 0 fp32, 1 bf16, 2 fp16
 
 // ---- distill.hip -----------------------------------------------------------------------

@@ -54,8 +54,8 @@ def _lengths(key_lengths, B, T, device):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_floats(B, U, T, H, Hkv, D):
-    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D))
+def _workspace_floats(B, U, T, H, Hkv, D, code):
+    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D, dtype=code))
 
 
 def _forward(query, key, value, key_lengths, scale, want_lse):
@@ -77,7 +77,7 @@ def _forward(query, key, value, key_lengths, scale, want_lse):
     d = CrossAttentionDesc(B, U, T, H, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     out = torch.empty(qs, device=device, dtype=dtype)
     lse = torch.empty((B, U, H), device=device, dtype=torch.float32) if want_lse else None
-    n = _workspace_floats(B, U, T, H, Hkv, D)
+    n = _workspace_floats(B, U, T, H, Hkv, D, code)
     work = torch.empty(n, device=device, dtype=torch.float32) if n else None
     _cabi.call_on(device, lib().las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),

@@ -117,6 +117,10 @@ SHAPES = [  # B, U, T, H, Hkv, D
     (3, 1, 1500, 8, 8, 64),        # split over key ranges
     (3, 2, 2100, 8, 2, 128),
     (3, 1, 1031, 4, 4, 24),
+    (32, 70, 200, 8, 8, 128),      # wide heads in the 128-row / 128-key forms
+    (2, 150, 1500, 4, 2, 64),      # 128 rows and key ranges
+    (1, 100, 1100, 2, 2, 128),
+    (2, 9, 300, 4, 4, 96),         # key ranges of fp32 alone
 ]
 
 
