@@ -277,6 +277,7 @@ int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, in
  *   q (B,U,H,D), k / v (B,T,Hkv,D) of one type (dtype 0 fp32, 1 bf16, 2 fp16), any strides (in elements) with rows of D contiguous; row
  *   starts 16-byte aligned; D <= 128, a multiple of 16 bytes.  out / dout / dq (B,U,H,D) and dk / dv (B,T,Hkv,D) contiguous.
  *   lse (B,U,H) fp32: log2 of the sum of exp(s), or -inf; NULL in a forward that no backward follows.  Scores, softmax and sums are fp32.
+ *   Backward: dq NULL, or dk and dv NULL: that side is not formed (features of a Listener that is not trained).
  *   workspace of the forward: las_cross_attention_workspace_floats() floats (0: may be NULL), private to the call until its kernels have run.
  *   No atomics: results are the same from run to run.  Any stream, capturable.
  * ---------------------------------------------------------------------------------------------- */

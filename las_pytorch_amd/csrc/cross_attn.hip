@@ -785,14 +785,14 @@ template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
-// Backward: both sides wide where that makes two workgroups per CU, fp32 one (its narrow shape has a CU to itself too: 41 against 56 us at 32 x 128
+// Backward (a side whose gradients nobody wants is left out): both sides wide where that makes two workgroups per CU, fp32 one (its narrow shape has a CU to itself too: 41 against 56 us at 32 x 128
 // over 100 heads of 128; not where most of 128 rows would be empty), else both narrow.
 template <class T, int DP> int bwd_dp(const CrossAttnArgs& args, hipStream_t stream) {
     CrossAttnArgs a = args;
     const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
     const long n = bh * ((R + 127) / 128 + (a.T + 127) / 128);
     const bool wide = n >= 2 * CA_CUS || (sizeof(T) == 4 && R > 64 && n >= CA_CUS);
-    const long per = wide ? 128 : 64, rows = blocks_of(a, (R + per - 1) / per), keys = blocks_of(a, (a.T + per - 1) / per);
+    const long per = wide ? 128 : 64, rows = a.dq ? blocks_of(a, (R + per - 1) / per) : 0, keys = a.dk ? blocks_of(a, (a.T + per - 1) / per) : 0;
     if (rows + keys == 0) return LAS_OK;
     LAS_TRY(check_grid(rows + keys));
     a.longest_first = a.lens && a.B > 1 && a.B <= 64 && rows + keys > 2 * CA_CUS;

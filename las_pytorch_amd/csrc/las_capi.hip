@@ -1510,8 +1510,8 @@ int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, co
     LAS_TRY(cross_attention_check(d, q, k, v));
     if (d->B == 0) return LAS_OK;
     const bool rows = d->U > 0, keys = d->T > 0;
-    LAS_REQUIRE(!rows || (out && lse && dout && dq), "cross attention backward pointers");
-    LAS_REQUIRE(!keys || (dk && dv), "cross attention gradients");
+    LAS_REQUIRE(!rows || (out && lse && dout), "cross attention backward pointers");
+    LAS_REQUIRE(!dk == !dv && (dq || dk || !rows || !keys), "cross attention gradients: dq, or dk and dv, or all three");
     LAS_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "cross attention tensors: 16-byte aligned");
     CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
     a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;

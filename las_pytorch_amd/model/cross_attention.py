@@ -99,12 +99,16 @@ class _CrossAttentionFn(torch.autograd.Function):
         q, k, v, key_lengths, out, lse = ctx.saved_tensors
         dout = _aligned(dout.contiguous())
         device = q.device
-        dq = torch.empty_like(out)
-        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
-        dv = torch.empty_like(dk)
+        dq = dk = dv = None
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        if need_q:
+            dq = torch.empty_like(out)
+        if need_k or need_v:
+            dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+            dv = torch.empty_like(dk)
         _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+                      None if dq is None else dq.data_ptr(), None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr())
         return dq, dk, dv, None, None
 
 
@@ -115,8 +119,9 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
     ``h`` reads key head ``h // (H // Hkv)``); D a multiple of 16 bytes, at most 128.  ``key_lengths`` (B,) int32 / int64 on the device: the
     utterances' valid frames (clamped to [0, T]); the frames behind them are never read and get zero gradients, and an utterance without
     any gives zeros.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once) in query, key and value.
-    Scores, softmax and sums are fp32 whatever the type; an infinite value in a valid place gives NaN.  U = 1 is one decode step: the key range is split over the GPU where the batch
-    alone does not fill it.  Rows that are not contiguous or not 16-byte aligned are copied first."""
+    Scores, softmax and sums are fp32 whatever the type; an infinite value in a valid place gives NaN.  U = 1 is one decode step: the key
+    range is split over the GPU where the batch alone does not fill it.  Gradients that nobody asks for are not formed.  Rows that are not
+    contiguous or not 16-byte aligned are copied first."""
     if scale is not None:
         scale = float(scale)
         if not 0.0 < scale < math.inf:

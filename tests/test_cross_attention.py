@@ -231,12 +231,28 @@ def test_shared_encoder_states_sum_their_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 20, 90, 4, 2, 64), (40, 129, 131, 16, 8, 64)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_gradients_of_one_side(dtype, shape):
+    """A Listener that is not trained (dq alone), frozen decoder states (dk, dv alone): the bits of the full backward."""
+    q, k, v, dout, lengths = _inputs(dtype, *shape, seed=8)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    every = torch.autograd.grad(cross_attention(*leaves, lengths), leaves, dout)
+    for wanted in ((0,), (1, 2), (2,)):
+        xs = [x.detach().requires_grad_(i in wanted) for i, x in enumerate((q, k, v))]
+        got = torch.autograd.grad(cross_attention(*xs, lengths), [xs[i] for i in wanted], dout)
+        assert all(torch.equal(g, every[i]) for g, i in zip(got, wanted))
+
+
+@pytest.mark.gpu
 def test_empty_sizes():
     for B, U, T in ((0, 3, 5), (2, 0, 5), (2, 3, 0)):
         q, k, v = (torch.randn(B, n, 2, 32, device="cuda", requires_grad=True) for n in (U, T, T))
         out = cross_attention(q, k, v)
         grads = torch.autograd.grad(out.sum(), (q, k, v))
         assert out.shape == q.shape and not out.any() and not any(g.any() for g in grads)
+        (dk,) = torch.autograd.grad(cross_attention(q.detach(), k, v.detach()).sum(), (k,))
+        assert dk.shape == k.shape and not dk.any()
 
 
 @pytest.mark.gpu
@@ -331,6 +347,8 @@ def test_c_entry_refuses_before_it_launches():
         assert L.las_cross_attention_fwd(d, *ptrs, None, 4096, None, None, None) == 1
     assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, None, None, None, None) == 1
     assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, None, 4096, 4096, 4096, 4096, None) == 1
+    for grads in ((None, 4096, None), (4096, None, 4096), (None, None, None)):       # half of a side, nothing at all
+        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, *grads, None) == 1
     assert L.las_cross_attention_fwd(None, 4096, 4096, 4096, None, 4096, None, None, None) == 1
     assert L.las_cross_attention_workspace_floats(d) == 0
     assert L.las_cross_attention_workspace_floats(_cabi.CrossAttentionDesc(**{**good, "T": 4096})) > 0
