@@ -269,28 +269,60 @@ static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
 // Where a launch takes more than one round of the GPU (`a.longest_first`), an XCD's workgroups start in falling order of their utterances' lengths and
 // the XCDs take turns in that order, so that the last round fills up with the short ones (16 x 512 over ragged 1500: 259 -> 240 us a step).  A
 // permutation of the work for any placement of blocks.
+// TILED: the `per` workgroups lie along the keys, TILED keys each.  Those behind an utterance's end have only zeros to write and start after all others:
+// the shader engines of an XCD take its workgroups in turn, so that one that is done at once leaves its place empty until the turn comes round.
 struct Work { int i, b, kvh; bool any; };      // i: which of the `per` workgroups of (b, kvh)
-static __device__ __forceinline__ Work work_of(const CrossAttnArgs& a, int block, int per) {
-    const int local = block >> 3, at = (local / per) * 8 + (block & 7), n = a.B * a.Hkv;
-    Work w = {local % per, at / a.Hkv, at % a.Hkv, at < n};
-    if (!a.longest_first || !w.any) return w;
-    // the utterance whose length is the w.b-th largest (equal lengths by index); a lane for each of at most 64
+template <int TILED = 0> static __device__ __forceinline__ Work work_of(const CrossAttnArgs& a, int block, int per) {
+    const int local = block >> 3, n = a.B * a.Hkv, xcd = block & 7;
+    int at = local / per * 8 + xcd, i = local % per;
+    Work w = {i, at / a.Hkv, at % a.Hkv, at < n};
+    if (!a.longest_first) return w;
+    // the utterance whose length is the r-th largest (equal lengths by index) in lane r; a lane for each of at most 64
     const int lane = threadIdx.x & 63, mine = lane < a.B ? length_of(a, lane) : -1;
     int rank = 0;
     for (int j = 0; j < a.B; ++j) {
         const int other = __builtin_amdgcn_readlane(mine, j);
         rank += other > mine || (other == mine && j < lane) ? 1 : 0;
     }
-    w.b = __ffsll((long long)__ballot(lane < a.B && rank == w.b)) - 1;
+    const int sorted = __builtin_amdgcn_ds_permute((lane < a.B ? rank : lane) * 4, lane);
+    const int groups = (n + 7) / 8;
+    if (TILED > 0 && groups <= 64) {
+        // lane g: the XCD's g-th (utterance, key head), its tiles of keys and of zeros, and their sums up to here
+        const bool mine_any = lane < groups && lane * 8 + xcd < n;
+        const int b = __shfl(sorted, mine_any ? (lane * 8 + xcd) / a.Hkv : 0), len = __shfl(mine, b);
+        const int keys = mine_any ? (len + TILED - 1) / (TILED > 0 ? TILED : 1) : 0;
+        int upto = keys, zeros = mine_any ? per - keys : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o), y = __shfl_up(zeros, o);
+            if (lane >= o) { upto += x; zeros += y; }
+        }
+        const int all = __builtin_amdgcn_readlane(upto, 63), rest = local - all;
+        const bool zero = rest >= 0;
+        const unsigned long long past = __ballot(zero ? zeros > rest : upto > local);
+        if (past == 0) { w.any = false; return w; }
+        const int g = __ffsll((long long)past) - 1;
+        const int own = __builtin_amdgcn_readlane(keys, g), before = __builtin_amdgcn_readlane(zero ? zeros : upto, g) - (zero ? per - own : own);
+        at = g * 8 + xcd;
+        w = {zero ? own + rest - before : local - before, at / a.Hkv, at % a.Hkv, true};
+    }
+    if (w.any) w.b = __builtin_amdgcn_readlane(sorted, w.b);
     return w;
 }
 // blocks of a launch of `per` workgroups for each (utterance, key head)
 static long blocks_of(const CrossAttnArgs& a, long per) { return ((long)a.B * a.Hkv + 7) / 8 * 8 * per; }
 
 
-// Workgroups per CU that the registers are budgeted for (as many waves per SIMD): two where a workgroup's tiles fit 256 registers, else one.
+// Workgroups per CU that the registers are budgeted for (as many waves per SIMD): two where a workgroup's tiles fit 256 registers (18 of them to and from
+// scratch memory at 16-bit heads of 128 cost less than the second workgroup gives: backward of 16 x 1024 over 2048, 1614 -> 1161 us), else one.
 template <class T, int DP> constexpr int FWD_PER_CU = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
-template <class T, int DP> constexpr int BWD_PER_CU = (sizeof(T) == 2 && DP <= 64) || DP <= 32 ? 2 : 1;
+template <class T, int DP, int NW> constexpr int BWD_PER_CU = DP <= 32 || (sizeof(T) == 2 && DP <= 96) || (NW == 4 && (sizeof(T) == 2 || DP <= 64)) ? 2 : 1;
+// Tiles of 32 keys (rows) that a wide workgroup's waves take at a time.  Two halve the barriers, one leaves registers for another wave per SIMD: forward, 16-bit
+// heads of 64 (16 x 512 over ragged 1500: 55 -> 52 us; heads of 32 have four waves either way, 113 against 127 us at 16 x 1024 over 2048, heads of 96 three
+// against two, 254 against 261); backward, all but the smallest (heads of 64: 590 -> 557 us, of 96: 1320 -> 884; fp32 heads of 64, 16 x 512 over 1000: 399 -> 316;
+// heads of 32: 362 against 395).  One of fp32 is three planes.
+template <class T, int DP> constexpr int DEEP_FWD = (sizeof(T) == 4 && DP > 64) || (sizeof(T) == 2 && DP == 64) ? 1 : 2;
+template <class T, int DP> constexpr int DEEP_BWD = DP > 32 ? 1 : 2;
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 // Four waves: NWQ of them side by side over rows (32 each), NWK over keys (KT tiles of 32 of every key tile each).
@@ -610,7 +642,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
     float* sD = sL + BR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
-    const Work w = work_of(a, block, ntiles);
+    const Work w = work_of<32 * NWK>(a, block, ntiles);
     if (!w.any) return;
     const int tile = w.i, b = w.b, kvh = w.kvh;
     const int len = length_of(a, b);
@@ -637,8 +669,8 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
             at.next();
             ls.next();
         };
-        // (a fp32 tile of wide heads is asked for when it is stored: held through the products it would not fit the registers)
-        constexpr bool EARLY = DP <= 64 || (sizeof(T) == 2 && NWR == 1);
+        // (a tile of wider heads is asked for when it is stored: held through the products it would cost a wave per SIMD, which hides the wait better)
+        constexpr bool EARLY = DP <= 32;
         if (EARLY) fetch();
         Frag<T> kf[G::NCH], vf[G::NCH];
 #pragma unroll
@@ -737,7 +769,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
 
 // One launch: the side whose workgroups take longer first (`keys_first`, else the row side's), its `first` blocks before the other's.
 template <class T, int DP, int NW, int DEPTH>
-__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int first, int keys_first) {
+__global__ __launch_bounds__(CA_THREADS, (BWD_PER_CU<T, DP, NW>)) void cross_attn_bwd_kernel(CrossAttnArgs a, int first, int keys_first) {
     constexpr int A = DKV_BYTES<T, DP, NW, 4 / NW, DEPTH>(), B = DQ_BYTES<T, DP, NW, 4 / NW, DEPTH>();
     __shared__ __attribute__((aligned(16))) char smem[A > B ? A : B];
     const bool second = (int)blockIdx.x >= first;
@@ -772,13 +804,12 @@ template <class K> int launch(K kernel, long grid, CrossAttnArgs a, hipStream_t 
 // the key (row) tile too and joined at the end: 64 rows, in the forward of small 16-bit heads 32.  (32 rows in the backward, or of wide heads, hold
 // tiles of 128 of the other side: one workgroup to a CU, 20 against 12.5 us at 8 x 128 over 375 heads of 64, 70 against 27 at 4 x 400 over 500 heads of 96.)
 template <class T, int DP> constexpr int NARROW = sizeof(T) == 4 || DP > 64 ? 2 : 1;
-template <class T, int DP> constexpr int DEEP = sizeof(T) == 4 && DP > 64 ? 1 : 2;      // tiles of 32 per pass of the wide shape
 
 template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream) {
     constexpr int NQ = NARROW<T, DP>;
     const long R = (long)a.U * (a.H / a.Hkv);
     int rc;
-    if (fwd_wide(a.B, a.U, a.T, a.H, a.Hkv)) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, DEEP<T, DP>>, blocks_of(a, a.nsplit * ((R + 127) / 128)), a, stream);
+    if (fwd_wide(a.B, a.U, a.T, a.H, a.Hkv)) rc = launch(cross_attn_fwd_kernel<T, DP, 4, 1, DEEP_FWD<T, DP>>, blocks_of(a, a.nsplit * ((R + 127) / 128)), a, stream);
     else rc = launch(cross_attn_fwd_kernel<T, DP, NQ, 4 / NQ, 1>, blocks_of(a, a.nsplit * ((R + 32 * NQ - 1) / (32 * NQ))), a, stream);
     if (rc != LAS_OK || a.nsplit == 1) return rc;
     const long items = (long)a.B * a.U * a.H * (a.D / 4);
@@ -798,7 +829,7 @@ template <class T, int DP> int bwd_dp(const CrossAttnArgs& args, hipStream_t str
     a.longest_first = a.lens && a.B > 1 && a.B <= 64 && rows + keys > 2 * CA_CUS;
     // (a workgroup of the key side goes over the rows in 16 products a tile, one of the row side over the keys in 12)
     const int keys_first = R * 4 >= (long)a.T * 3, first = (int)(keys_first ? keys : rows);
-    if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
+    if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP_BWD<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
     else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 2, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
     LAS_LAUNCH_CHECK();
     return LAS_OK;
