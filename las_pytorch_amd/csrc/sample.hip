@@ -419,32 +419,44 @@ template <int NT> static __device__ __forceinline__ u64 cut_in_list(const Weighe
 }
 
 // The draw within [lo, hi) of a row, of the candidates not behind the cut: target as in reach, total for the share.  Ranges of the range, one per
-// wave, until every thread has one index.
+// wave, until every thread has one index.  total = 0: neither is known yet, the range is the whole row; the first ranges' masses give both.
 template <int NT, class T>
-static __device__ void draw_range(const SampleArgs& a, int row, const T* z, const Weigher& w, u64 cut, u64 least, int lo, int hi, u64 target, u64 total, Shared& s) {
+static __device__ void draw_range(const SampleArgs& a, int row, const T* z, const Limits& lim, const Weigher& w, u64 cut, u64 least, int lo, int hi, u64 target, u64 total,
+                                  Shared& s) {
     constexpr int NW = NT / 64;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    auto mass_at = [&](int i) {
-        const float x = logit_at(z, i);
+    auto mass_of = [&](float x, int i) {
         if (x == -INFINITY || place_of(x, i) < cut) return (u64)0;
         const u64 f = w.fixed(x);
         return f >= least ? f : (u64)0;
     };
-    while (hi - lo > NT) {
+    bool first = total == 0;
+    while (hi - lo > NT || first) {
         const int per = (hi - lo + NW - 1) / NW, x0 = min(hi, lo + wave * per), x1 = min(hi, x0 + per);
         u64 m = 0;
-        for (int i = x0 + lane; i < x1; i += 64) m += mass_at(i);
+        float next = x0 + lane < x1 ? logit_at(z, x0 + lane) : 0.f;
+#pragma unroll 1
+        for (int i = x0 + lane; i < x1; i += 64) {
+            const float x = next;
+            next = i + 64 < x1 ? logit_at(z, i + 64) : 0.f;
+            m += mass_of(x, i);
+        }
         m = wave_sum(m);
         __syncthreads();
         if (lane == 0) s.mass[wave] = m;
         __syncthreads();
+        if (first) {
+            for (int i = 0; i < NW; ++i) total += s.mass[i];
+            target = lim.goal(total);
+            first = false;
+        }
         int part; u64 before;
         reach<NT>(NW, target, [&](int i) { return s.mass[i]; }, s, part, before);
         target -= before;
         lo = min(hi, lo + part * per);
         hi = min(hi, lo + per);
     }
-    const u64 x = lo + tid < hi ? mass_at(lo + tid) : 0;
+    const u64 x = lo + tid < hi ? mass_of(logit_at(z, lo + tid), lo + tid) : 0;
     u64 all;
     const u64 incl = block_scan<NT>(x, all, s);
     if (incl - x < target && target <= incl) answer(a, row, lo + tid, share(x, total));
@@ -523,15 +535,7 @@ template <class T, int NT> static __device__ __attribute__((noinline)) void row_
         if (here <= SM_CAP) cut = cut_in_list<NT>(w, true, target - before, gather(bin, bin), s);
         else cut = cut_in_row<NT>(z, V, w, cut, true, target, s);
     }
-    const u64 least = lim.least(w.unit);
-    u64 m = 0;
-    each_logit<NT>(z, 0, V, [&](float x, int i) {
-        if (x == -INFINITY || place_of(x, i) < cut) return;
-        const u64 f = w.fixed(x);
-        if (f >= least) m += f;
-    });
-    const u64 total = block_sum<NT>(m, s);
-    draw_range<NT>(a, row, z, w, cut, least, 0, V, lim.goal(total), total, s);
+    draw_range<NT>(a, row, z, lim, w, cut, lim.least(w.unit), 0, V, 0, 0, s);
 }
 
 // top_k of a row without a pass that counts: of the maxima that the threads found in their shares of the row, the top_k-th largest has at least top_k
@@ -844,13 +848,13 @@ template <class T> __global__ __launch_bounds__(SL_THREADS) void sample_draw_ker
     u64 before;
     int part;
     reach<NT>(chunks, goal, [&](int i) { return s.mass[i]; }, s, part, before);
-    draw_range<NT>(a, row, z, w, cut, least, part * SM_CHUNK, min(V, (part + 1) * SM_CHUNK), goal - before, total, s);
+    draw_range<NT>(a, row, z, lim, w, cut, least, part * SM_CHUNK, min(V, (part + 1) * SM_CHUNK), goal - before, total, s);
 }
 
 static_assert(SM_CHUNKS <= SM_BINS, "the draw keeps the chunks' masses where the histogram was");
 
 template <class T> int by_size(const SampleArgs& a, void* workspace, hipStream_t stream) {
-    // (top_k from one scalar: a workgroup finds a short list in two reads of the row, 64 rows of 32000: 34 us in slices, 16 us here)
+    // (top_k from one scalar: a workgroup finds a short list in two reads of the row, 64 rows of 32000: 34 us in slices, 15 us here)
     const int S = a.top_k > 1 && a.top_k <= 512 && !a.top_k_rows ? 1 : sample_slices(a.B, a.V);
     if (a.V <= 64) {
         hipLaunchKernelGGL(sample_wave_kernel<T>, dim3((unsigned)((a.B + 3) / 4)), dim3(SW_THREADS), 0, stream, a);
