@@ -316,12 +316,18 @@ int las_letter_error_rate(const float* logp, int64_t stride_u, int64_t stride_b,
  *   [0, V) is absent, a class named twice counts with both entries, a row without entries adds nothing.
  *   lengths int32 (B) on the device (clamped to [0, U]) or NULL: all U steps.
  *   loss: 1 float (needs scratch: B U floats), or NULL.  dlogits: gradient of the loss in the logits' type, addressed like them with
- *   dstride_*, or NULL; multiplied by *upstream (device) unless that is NULL.  One pass over the logits either way; no atomics. */
-int las_distill_loss(const void* logits, int64_t stride_u, int64_t stride_b, int dtype, const void* index, int index_64, const void* teacher,
-                     int teacher_dtype, const int32_t* lengths, int B, int U, int V, int K, float temperature, float* loss, void* dlogits,
-                     int64_t dstride_u, int64_t dstride_b, const float* upstream, float* scratch, void* stream);
-/* x[0..n) *= *factor (device), nothing read or written when the factor is 1: the backward of a loss whose forward left its gradient. */
-int las_scale_unless_one(void* x, size_t n, int dtype, const float* factor, void* stream);
+ *   dstride_*, or NULL; multiplied by *upstream (device) unless that is NULL.  One pass over the logits either way; no atomics.
+ * las_distill_grad_unless_one: the backward of a loss whose forward left its gradient.  dlogits holds it for a factor of one; nothing happens where
+ *   *upstream is one, else it is formed anew with the factor inside (rounded to the logits' type once: a scaled loss keeps what fp16 would have lost). */
+typedef struct las_distill_desc {
+    int B, U, V, K, dtype, teacher_dtype, index_64;
+    float temperature;
+    int64_t stride_b, stride_u, dstride_b, dstride_u;
+} las_distill_desc;
+int las_distill_loss(const las_distill_desc* d, const void* logits, const void* index, const void* teacher, const int32_t* lengths, float* loss,
+                     void* dlogits, const float* upstream, float* scratch, void* stream);
+int las_distill_grad_unless_one(const las_distill_desc* d, const void* logits, const void* index, const void* teacher, const int32_t* lengths,
+                                void* dlogits, const float* upstream, void* stream);
 
 /* Global-norm clip + Adam step on the flat gradient buffer in two launches: torch.nn.utils.clip_grad_norm_(params, max_norm)
  * followed by torch.optim.Adam.step() (amsgrad off, weight_decay 0) — reference solver/solver.py:96-97, train.py:82.

@@ -50,6 +50,11 @@ class CrossAttentionDesc(C.Structure):
                 + [(n, C.c_int64) for n in ("q_b", "q_u", "q_h", "k_b", "k_t", "k_h", "v_b", "v_t", "v_h")])
 
 
+class DistillDesc(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("B", "U", "V", "K", "dtype", "teacher_dtype", "index_64")] + [("temperature", C.c_float)]
+                + [(n, C.c_int64) for n in ("stride_b", "stride_u", "dstride_b", "dstride_u")])
+
+
 # name -> (restype, argtypes); every symbol include/las_hip.h declares
 PROTOTYPES = {
     "las_abi_version": (C.c_int, []),
@@ -97,9 +102,8 @@ PROTOTYPES = {
     "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 11),
     "las_ls_loss": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _f, _f, C.c_int64,
                               C.c_int64, _f, _f]),
-    "las_distill_loss": (C.c_int, [_f, C.c_int64, C.c_int64, C.c_int, _f, C.c_int, _f, C.c_int, _f] + [C.c_int] * 4
-                         + [C.c_float, _f, _f, C.c_int64, C.c_int64, _f, _f, _f]),
-    "las_scale_unless_one": (C.c_int, [_f, C.c_size_t, C.c_int, _f, _f]),
+    "las_distill_loss": (C.c_int, [C.POINTER(DistillDesc)] + [_f] * 9),
+    "las_distill_grad_unless_one": (C.c_int, [C.POINTER(DistillDesc)] + [_f] * 7),
     "las_letter_error_rate": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, _f, _f, _f]),
     "las_collate_pad": (C.c_int, [_f, _f, _f, _f] + [C.c_int] * 5 + [_f, _f, _f]),
     "las_comm_uid": (C.c_int, [C.c_char_p]),

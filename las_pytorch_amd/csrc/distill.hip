@@ -70,6 +70,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     float* sp = dyn;                             // K: teacher probabilities
     int* si = (int*)(dyn + a.K);                 // K: classes
     __shared__ float red[2 * NT / 64];
+    if (a.unless_one && *a.upstream == 1.f) return;
     const int tid = threadIdx.x;
     const long row = blockIdx.x;
     const int b = (int)(row / a.U), u = (int)(row - (long)b * a.U);
@@ -217,25 +218,6 @@ __global__ __launch_bounds__(SUM_THREADS) void distill_sum_kernel(const float* _
     }
 }
 
-// x *= *factor, not touched when the factor is one (the seed of an ordinary backward)
-template <class T> __global__ __launch_bounds__(256) void scale_unless_one_kernel(T* __restrict__ x, long n, const float* __restrict__ factor) {
-    const float f = *factor;
-    if (f == 1.f) return;
-    using V = typename Vec<T>::V;
-    constexpr int EL = Vec<T>::EL;
-    const long step = (long)gridDim.x * 256 * EL;
-    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * EL; i < n; i += step) {
-        if (i + EL <= n) {
-            V y = *(V*)(x + i);
-#pragma unroll
-            for (int e = 0; e < EL; ++e) y[e] = (T)((float)y[e] * f);
-            *(V*)(x + i) = y;
-        } else {
-            for (long j = i; j < n; ++j) x[j] = (T)((float)x[j] * f);
-        }
-    }
-}
-
 template <class T, int NT, int NV> int launch(const DistillArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((distill_kernel<T, NT, NV>), dim3((unsigned)((long)a.B * a.U)), dim3(NT), (size_t)a.K * 8, stream, a);
     LAS_LAUNCH_CHECK();
@@ -263,16 +245,6 @@ int distill(const DistillArgs& args, int dtype, float* loss, hipStream_t stream)
     const int rc = dtype == 0 ? by_size<float>(a, stream) : dtype == 1 ? by_size<__bf16>(a, stream) : by_size<_Float16>(a, stream);
     if (rc != LAS_OK || !loss) return rc;
     hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(SUM_THREADS), 0, stream, a.rows, (long)a.B * a.U, loss);
-    LAS_LAUNCH_CHECK();
-    return LAS_OK;
-}
-
-int scale_unless_one(void* x, size_t n, int dtype, const float* factor, hipStream_t stream) {
-    const size_t el = dtype == 0 ? 4 : 8, pieces = (n + el - 1) / el;
-    const unsigned grid = (unsigned)(pieces < 256 * 2048 ? (pieces + 255) / 256 : 2048);
-    if (dtype == 0) hipLaunchKernelGGL(scale_unless_one_kernel<float>, dim3(grid), dim3(256), 0, stream, (float*)x, (long)n, factor);
-    else if (dtype == 1) hipLaunchKernelGGL(scale_unless_one_kernel<__bf16>, dim3(grid), dim3(256), 0, stream, (__bf16*)x, (long)n, factor);
-    else hipLaunchKernelGGL(scale_unless_one_kernel<_Float16>, dim3(grid), dim3(256), 0, stream, (_Float16*)x, (long)n, factor);
     LAS_LAUNCH_CHECK();
     return LAS_OK;
 }

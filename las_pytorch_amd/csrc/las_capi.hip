@@ -1397,27 +1397,31 @@ int las_ls_loss(const float* logp, int64_t stride_u, int64_t stride_b, const int
                    dstride_u, dstride_b, (hipStream_t)stream);
 }
 
-int las_distill_loss(const void* logits, int64_t stride_u, int64_t stride_b, int dtype, const void* index, int index_64, const void* teacher,
-                     int teacher_dtype, const int32_t* lengths, int B, int U, int V, int K, float temperature, float* loss, void* dlogits,
-                     int64_t dstride_u, int64_t dstride_b, const float* upstream, float* scratch, void* stream) {
-    LAS_REQUIRE(logits && index && teacher, "distillation pointers");
-    LAS_REQUIRE(dtype >= 0 && dtype <= 2 && teacher_dtype >= 0 && teacher_dtype <= 2, "distillation dtype");
-    LAS_REQUIRE(B > 0 && U > 0 && V > 0 && V < (1 << 30) && K > 0 && K <= 1024 && (int64_t)B * U < 0x7fffffffLL, "distillation dims (1 <= K <= 1024)");
-    LAS_REQUIRE(temperature > 0.f && temperature < 1e30f, "distillation temperature: positive");
+static int distill_call(const las_distill_desc* d, const void* logits, const void* index, const void* teacher, const int32_t* lengths, float* loss,
+                        void* dlogits, const float* upstream, int unless_one, float* scratch, void* stream) {
+    LAS_REQUIRE(d && logits && index && teacher, "distillation pointers");
+    LAS_REQUIRE(d->dtype >= 0 && d->dtype <= 2 && d->teacher_dtype >= 0 && d->teacher_dtype <= 2, "distillation dtype");
+    LAS_REQUIRE(d->B > 0 && d->U > 0 && d->V > 0 && d->V < (1 << 30) && d->K > 0 && d->K <= 1024 && (int64_t)d->B * d->U < 0x7fffffffLL,
+                "distillation dims (1 <= K <= 1024)");
+    LAS_REQUIRE(d->temperature > 0.f && d->temperature < 1e30f, "distillation temperature: positive");
     LAS_REQUIRE(loss || dlogits, "distillation outputs");
     LAS_REQUIRE(!loss || scratch, "distillation scratch");
+    LAS_REQUIRE(!unless_one || upstream, "distillation factor");
     DistillArgs a = {};
     a.z = logits; a.idx = index; a.t = teacher; a.dz = dlogits; a.rows = loss ? scratch : nullptr; a.lens = lengths; a.upstream = upstream;
-    a.z_b = stride_b; a.z_u = stride_u; a.dz_b = dstride_b; a.dz_u = dstride_u;
-    a.B = B; a.U = U; a.V = V; a.K = K; a.t_dtype = teacher_dtype; a.idx64 = index_64; a.tau = temperature;
-    return distill(a, dtype, loss, (hipStream_t)stream);
+    a.z_b = d->stride_b; a.z_u = d->stride_u; a.dz_b = d->dstride_b; a.dz_u = d->dstride_u;
+    a.B = d->B; a.U = d->U; a.V = d->V; a.K = d->K; a.t_dtype = d->teacher_dtype; a.idx64 = d->index_64; a.unless_one = unless_one; a.tau = d->temperature;
+    return distill(a, d->dtype, loss, (hipStream_t)stream);
 }
 
-int las_scale_unless_one(void* x, size_t n, int dtype, const float* factor, void* stream) {
-    LAS_REQUIRE(dtype >= 0 && dtype <= 2, "scale dtype");
-    LAS_REQUIRE((x || n == 0) && factor, "scale pointers");
-    if (n == 0) return LAS_OK;
-    return scale_unless_one(x, n, dtype, factor, (hipStream_t)stream);
+int las_distill_loss(const las_distill_desc* d, const void* logits, const void* index, const void* teacher, const int32_t* lengths, float* loss,
+                     void* dlogits, const float* upstream, float* scratch, void* stream) {
+    return distill_call(d, logits, index, teacher, lengths, loss, dlogits, upstream, 0, scratch, stream);
+}
+
+int las_distill_grad_unless_one(const las_distill_desc* d, const void* logits, const void* index, const void* teacher, const int32_t* lengths,
+                                void* dlogits, const float* upstream, void* stream) {
+    return distill_call(d, logits, index, teacher, lengths, nullptr, dlogits, upstream, 1, nullptr, stream);
 }
 
 int las_letter_error_rate(const float* logp, int64_t stride_u, int64_t stride_b, const int64_t* labels_onehot, int U, int U_lab,

@@ -382,10 +382,10 @@ struct DistillArgs {
     const float* upstream;         // one factor of the gradient on the device; NULL: 1
     long z_b, z_u, dz_b, dz_u;
     int B, U, V, K, t_dtype, idx64, stream_out;
+    int unless_one;                // nothing to do where *upstream is one
     float tau;
 };
 int distill(const DistillArgs& a, int dtype, float* loss, hipStream_t stream);        // dtype 0 fp32, 1 bf16, 2 fp16
-int scale_unless_one(void* x, size_t n, int dtype, const float* factor, hipStream_t stream);
 
 // ---- sample.hip ------------------------------------------------------------------------
 // One token per row of logits (B,V).  *_rows: one value per row on the device, or NULL: the scalar.

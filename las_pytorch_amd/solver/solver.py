@@ -171,8 +171,8 @@ def label_smoothing_loss_backward_device(pred_y, labels_onehot_int64, label_smoo
 
 class _DistillationLoss(torch.autograd.Function):
     """``las_distill_loss``: the forward leaves the gradient of the loss beside its value (one pass over the logits), the first backward hands
-    it over, multiplied in place where its seed is not one; a further backward of a retained graph forms it again.  In a stream capture the
-    backward forms it always: replayed alone, it would multiply what it has multiplied before."""
+    it over, formed anew where its seed is not one (a seed that came after the rounding to 16 bits could not bring back what that had lost);
+    a further backward of a retained graph, or one under a stream capture, forms it always."""
 
     @staticmethod
     def forward(ctx, logits, index, teacher, lengths, temperature):
@@ -181,39 +181,46 @@ class _DistillationLoss(torch.autograd.Function):
             grad = torch.empty_like(logits)
             if grad.stride(2) != 1:
                 grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        loss = _distill(logits, index, teacher, lengths, temperature, True, grad, None)
+        loss, ctx.desc = _distill(logits, index, teacher, lengths, temperature, grad)
         ctx.save_for_backward(logits, index, teacher, lengths)
-        ctx.temperature, ctx.grad = temperature, grad
+        ctx.temperature, ctx.grad, ctx.strides = temperature, grad, logits.stride()
         return loss
 
     @staticmethod
     @_cabi.differentiable_once
     def backward(ctx, upstream):
         logits, index, teacher, lengths = ctx.saved_tensors
+        lens = None if lengths is None else lengths.data_ptr()
         grad = None
-        if not torch.cuda.is_current_stream_capturing():
+        if not torch.cuda.is_current_stream_capturing() and logits.stride() == ctx.strides:
             grad, ctx.grad = ctx.grad, None
         if grad is not None:
-            _cabi.call_on(grad.device, _cabi.lib().las_scale_unless_one, grad.data_ptr(), grad.numel(), _cabi.DTYPES[grad.dtype], upstream.data_ptr())
+            _cabi.call_on(grad.device, _cabi.lib().las_distill_grad_unless_one, ctx.desc, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), lens,
+                          grad.data_ptr(), upstream.data_ptr())
         else:
             grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-            _distill(logits, index, teacher, lengths, ctx.temperature, False, grad, upstream)
+            _cabi.call_on(grad.device, _cabi.lib().las_distill_loss, _distill_desc(logits, index, teacher, ctx.temperature, grad), logits.data_ptr(),
+                          index.data_ptr(), teacher.data_ptr(), lens, None, grad.data_ptr(), upstream.data_ptr(), None)
         return grad, None, None, None, None
 
 
-def _distill(logits, index, teacher, lengths, temperature, want_loss, grad, upstream):
+def _distill_desc(logits, index, teacher, temperature, grad):
     B, U, V = logits.shape
-    dev = logits.device
-    loss = torch.empty((), device=dev, dtype=torch.float32) if want_loss else None
-    rows = torch.empty(B * U, device=dev, dtype=torch.float32) if want_loss else None
-    gb, gu = (0, 0) if grad is None else grad.stride()[:2]
     zb, zu, _ = logits.stride()
-    _cabi.call_on(dev, _cabi.lib().las_distill_loss, logits.data_ptr(), zu, zb, _cabi.DTYPES[logits.dtype],
-                  index.data_ptr(), index.dtype == torch.int64, teacher.data_ptr(), _cabi.DTYPES[teacher.dtype],
-                  None if lengths is None else lengths.data_ptr(), B, U, V, index.shape[2], temperature,
-                  loss.data_ptr() if want_loss else None, None if grad is None else grad.data_ptr(),
-                  gu, gb, None if upstream is None else upstream.data_ptr(), rows.data_ptr() if want_loss else None)
-    return loss
+    gb, gu = (0, 0) if grad is None else grad.stride()[:2]
+    return _cabi.DistillDesc(B, U, V, index.shape[2], _cabi.DTYPES[logits.dtype], _cabi.DTYPES[teacher.dtype], index.dtype == torch.int64, temperature,
+                             zb, zu, gb, gu)
+
+
+def _distill(logits, index, teacher, lengths, temperature, grad):
+    """The loss, its gradient into ``grad`` (or None), and the call's descriptor."""
+    dev = logits.device
+    loss = torch.empty((), device=dev, dtype=torch.float32)
+    rows = torch.empty(logits.shape[:2], device=dev, dtype=torch.float32)
+    desc = _distill_desc(logits, index, teacher, temperature, grad)
+    _cabi.call_on(dev, _cabi.lib().las_distill_loss, desc, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(),
+                  None if lengths is None else lengths.data_ptr(), loss.data_ptr(), None if grad is None else grad.data_ptr(), None, rows.data_ptr())
+    return loss, desc
 
 
 def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=1.0, lengths=None):
@@ -260,7 +267,7 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     teacher_index, teacher_logits = teacher_index.contiguous(), teacher_logits.contiguous()
     if torch.is_grad_enabled() and pred_y.requires_grad:
         return _DistillationLoss.apply(pred_y, teacher_index, teacher_logits, lengths, temperature)
-    return _distill(pred_y, teacher_index, teacher_logits, lengths, temperature, True, None, None)
+    return _distill(pred_y, teacher_index, teacher_logits, lengths, temperature, None)[0]
 
 
 # --------------------------------------------------------------------------------------------------

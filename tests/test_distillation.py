@@ -169,6 +169,16 @@ def test_seeds_and_retained_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=lambda t: str(t)[6:])
+def test_scaled_losses(dtype):
+    """Seeds of a scaled or weighted loss: the gradient is rounded to its type once, with the seed inside.  (V = 4097: most unscaled entries lie below
+    what fp16 can hold; 4 x 7 steps: the largest entry, 65536 / 4, lies within it.)"""
+    z, index, teacher, lengths = _case(dtype, 4, 7, 4097, 8, seed=9)
+    for seed in (65536.0, -2.5, 1 / 3, 2.0 ** -12):
+        _check(z, index, teacher, 1.0, lengths, seed)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """Against central differences of the formula in 64 bits, along a random direction (step 1e-5)."""
     z, index, teacher, lengths = _case(torch.float32, 2, 3, 50, 7, seed=6)
@@ -282,19 +292,22 @@ def test_refusals():
 def test_c_entry_refuses_before_it_launches():
     """Status 1 and a message, nothing touched (runs without a GPU)."""
     L = _cabi.lib()
-    names = ["logits", "su", "sb", "dtype", "index", "i64", "teacher", "tdtype", "lengths", "B", "U", "V", "K", "tau", "loss", "dlogits", "dsu", "dsb",
-             "upstream", "scratch", "stream"]
-    good = dict(logits=4096, su=8, sb=8, dtype=0, index=4096, i64=1, teacher=4096, tdtype=0, lengths=None, B=1, U=1, V=8, K=2, tau=1.0, loss=4096,
-                dlogits=4096, dsu=8, dsb=8, upstream=None, scratch=4096, stream=None)
-    for change in (dict(logits=None), dict(index=None), dict(teacher=None), dict(dtype=3), dict(dtype=-1), dict(tdtype=3), dict(B=0), dict(U=0), dict(V=0),
-                   dict(V=1 << 30), dict(K=0), dict(K=1025), dict(tau=0.0), dict(tau=-1.0), dict(tau=math.nan), dict(tau=math.inf),
-                   dict(loss=None, dlogits=None), dict(scratch=None), dict(B=1 << 20, U=1 << 20)):
-        assert L.las_distill_loss(*({**good, **change}[n] for n in names)) == 1, change
+    shape = dict(B=1, U=1, V=8, K=2, dtype=0, teacher_dtype=0, index_64=1, temperature=1.0, stride_b=8, stride_u=8, dstride_b=8, dstride_u=8)
+    names = ["logits", "index", "teacher", "lengths", "loss", "dlogits", "upstream", "scratch", "stream"]
+    good = dict(logits=4096, index=4096, teacher=4096, lengths=None, loss=4096, dlogits=4096, upstream=4096, scratch=4096, stream=None)
+    for change in (dict(dtype=3), dict(dtype=-1), dict(teacher_dtype=3), dict(B=0), dict(U=0), dict(V=0), dict(V=1 << 30), dict(K=0), dict(K=1025),
+                   dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(B=1 << 20, U=1 << 20)):
+        d = _cabi.DistillDesc(**{**shape, **change})
+        assert L.las_distill_loss(d, *(good[n] for n in names)) == 1, change
+        assert L.las_distill_grad_unless_one(d, *(good[n] for n in names if n not in ("loss", "scratch"))) == 1, change
         assert b"distillation" in L.las_last_error()
-    assert L.las_scale_unless_one(None, 4, 0, 4096, None) == 1
-    assert L.las_scale_unless_one(4096, 4, 7, 4096, None) == 1
-    assert L.las_scale_unless_one(4096, 4, 0, None, None) == 1
-    assert L.las_scale_unless_one(None, 0, 0, 4096, None) == 0
+    d = _cabi.DistillDesc(**shape)
+    for change in (dict(logits=None), dict(index=None), dict(teacher=None), dict(loss=None, dlogits=None), dict(scratch=None)):
+        assert L.las_distill_loss(d, *({**good, **change}[n] for n in names)) == 1, change
+        assert b"distillation" in L.las_last_error()
+    for change in (dict(logits=None), dict(index=None), dict(teacher=None), dict(dlogits=None), dict(upstream=None)):
+        assert L.las_distill_grad_unless_one(d, *({**good, **change}[n] for n in names if n not in ("loss", "scratch"))) == 1, change
+    assert L.las_distill_loss(None, *(good[n] for n in names)) == 1
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         distillation_loss_device(torch.zeros(1, 1, 4), torch.zeros(1, 1, 2, dtype=torch.int64), torch.zeros(1, 1, 2))
 
