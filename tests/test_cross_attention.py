@@ -5,6 +5,7 @@ probabilities and absolute values taken inside every sum:
   e    relative error of one probability: the score is a D-term fp32 sum of |q||k| (D + 4 roundings at 2^-24 of the sum of absolute
        values), twice (numerator and normaliser), plus the exponential's argument and value;
   out  h |out| + (h + e + T 2^-24) sum_j P |v|                        (P rounded to the type, T-term sum, output rounded)
+  e    in the backward also 2 ln T 2^-24: P = 2^(s - lse), lse is up to log2 T beside the scores, and it and the difference are each rounded at that size
   ds   h |ds| + P (E_dp + E_D) + e P (|dp| + |D|),  E_dp = D 2^-24 |do||v|,  E_D = (h + D 2^-24) sum |do||out|  (D from the rounded out)
   fp16 only: what is rounded to it below 2^-14 is off by up to half a subnormal step, 2^-25 (``sub``): each ds; each P, which the kernels form
        too large, by 2^9 in the forward, 2^14 in the backward: by 2^-34 of the row's largest (P is taken relative to a maximum of the row's scores), 2^-39
@@ -52,6 +53,7 @@ def reference(q, k, v, lengths, dout=None, scale=None):
     ds = P * (dp - delta)
     E_dp = D * f32 * dO.abs() @ V.abs().transpose(2, 3)
     E_D = (dO.abs() * E_out).sum(-1, keepdim=True) + D * f32 * (dO.abs() * out.abs()).sum(-1, keepdim=True)
+    rel = rel + 2 * math.log(max(T, 2)) * f32
     E_ds = h * ds.abs() + P * (E_dp + E_D) + (rel + 4 * f32) * P * (dp.abs() + delta.abs()) + sub * keep
     E_p = (h + rel) * P + sub * 2.0 ** -14 * keep
     share = lambda x: x.reshape(B, Hkv, H // Hkv, T, D).sum(2).permute(0, 2, 1, 3)      # noqa: E731
