@@ -278,7 +278,8 @@ int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, in
  *   starts 16-byte aligned; D <= 128, a multiple of 16 bytes.  out / dout / dq (B,U,H,D) and dk / dv (B,T,Hkv,D) contiguous.
  *   lse (B,U,H) fp32: log2 of the sum of exp(s), or -inf; NULL in a forward that no backward follows.  Scores, softmax and sums are fp32.
  *   Backward: dq NULL, or dk and dv NULL: that side is not formed (features of a Listener that is not trained).
- *   workspace of the forward: las_cross_attention_workspace_floats() floats (0: may be NULL), private to the call until its kernels have run.
+ *   workspace: las_cross_attention_workspace_floats() floats in the forward, _bwd_workspace_floats() in the backward (0: may be NULL), private to the
+ *   call until its kernels have run.
  *   No atomics: results are the same from run to run.  Any stream, capturable.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct las_cross_attention_desc {
@@ -287,10 +288,11 @@ typedef struct las_cross_attention_desc {
     int64_t q_b, q_u, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
 } las_cross_attention_desc;
 size_t las_cross_attention_workspace_floats(const las_cross_attention_desc* d);
+size_t las_cross_attention_bwd_workspace_floats(const las_cross_attention_desc* d);
 int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
                             void* out, float* lse, float* workspace, void* stream);
 int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
-                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* stream);
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* workspace, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Caller-side contract on device (the code that CALLS the hot path, reference solver/solver.py).

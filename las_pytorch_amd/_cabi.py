@@ -98,8 +98,9 @@ PROTOTYPES = {
     "las_sample_tokens": (C.c_int, [_f, C.c_int64, C.c_int, C.c_int, C.c_int, _f, C.c_double, C.c_int, C.c_double, C.c_double] + [_f] * 8),
     "las_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "las_cross_attention_workspace_floats": (C.c_size_t, [C.POINTER(CrossAttentionDesc)]),
+    "las_cross_attention_bwd_workspace_floats": (C.c_size_t, [C.POINTER(CrossAttentionDesc)]),
     "las_cross_attention_fwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 8),
-    "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 11),
+    "las_cross_attention_bwd": (C.c_int, [C.POINTER(CrossAttentionDesc)] + [_f] * 12),
     "las_ls_loss": (C.c_int, [_f, C.c_int64, C.c_int64, _f, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _f, _f, C.c_int64,
                               C.c_int64, _f, _f]),
     "las_distill_loss": (C.c_int, [C.POINTER(DistillDesc)] + [_f] * 9),

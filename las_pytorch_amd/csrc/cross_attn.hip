@@ -229,14 +229,15 @@ template <int EL, int ROWS, int P> struct RowWalk {
     static constexpr int N = (ROWS * P + CA_THREADS - 1) / CA_THREADS;
     long a[N], b[N], step_a, step_b, wrap_a, wrap_b;
     int g[N], row0, rest, share, ch, row;
-    __device__ __forceinline__ RowWalk(long su_a, long sg_a, long su_b, long sg_b, int share_, int tid) : row0(0), share(share_), ch(tid % P), row(tid / P) {
+    __device__ __forceinline__ RowWalk(long su_a, long sg_a, long su_b, long sg_b, int share_, int from, int tid)
+        : row0(from), share(share_), ch(tid % P), row(tid / P) {
         static_assert(CA_THREADS % P == 0, "a thread keeps its place in the rows");
         rest = ROWS % share;
         step_a = ROWS / share * su_a + rest * sg_a; wrap_a = su_a - share * sg_a;
         step_b = ROWS / share * su_b + rest * sg_b; wrap_b = su_b - share * sg_b;
 #pragma unroll
         for (int v = 0; v < N; ++v) {
-            const int n = row + v * (CA_THREADS / P), u = n / share;
+            const int n = from + row + v * (CA_THREADS / P), u = n / share;
             g[v] = n - u * share;
             a[v] = u * su_a + g[v] * sg_a + ch * EL;
             b[v] = u * su_b + g[v] * sg_b + ch * EL;
@@ -309,6 +310,12 @@ template <int TILED = 0> static __device__ __forceinline__ Work work_of(const Cr
     if (w.any) w.b = __builtin_amdgcn_readlane(sorted, w.b);
     return w;
 }
+// the part-th of n ranges of [0, length): whole tiles of 32
+struct Range { int begin, end; };
+static __device__ __forceinline__ Range range_of(int length, int n, int part) {
+    const int per = ((length + n - 1) / n + 31) & ~31, begin = min(length, part * per);
+    return {begin, min(length, begin + per)};
+}
 // blocks of a launch of `per` workgroups for each (utterance, key head)
 static long blocks_of(const CrossAttnArgs& a, long per) { return ((long)a.B * a.Hkv + 7) / 8 * 8 * per; }
 
@@ -344,8 +351,8 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
     if (!w.any) return;
     const int tile = w.i % ntiles, split = w.i / ntiles, b = w.b, kvh = w.kvh;
     const int len = length_of(a, b);
-    const int per = ((len + a.nsplit - 1) / a.nsplit + 31) & ~31;
-    const int begin = min(len, split * per), end = min(len, begin + per);
+    const Range keys = range_of(len, a.nsplit, split);
+    const int begin = keys.begin, end = keys.end;
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
     const T* v = (const T*)a.v + b * a.v_b + kvh * a.v_h;
@@ -514,6 +521,22 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnAr
     if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
 }
 
+// four results of a type, or of fp32 where they are one range's
+template <class T> static __device__ __forceinline__ void put(float* part, T* to, f32x4 y) {
+    using V4 = __attribute__((ext_vector_type(4))) T;
+    if (part) *(f32x4*)part = y;
+    else *(V4*)to = __builtin_convertvector(y, V4);
+}
+// the sum of n ranges' results of `count` fours each, in their order
+template <class T> __global__ __launch_bounds__(CA_THREADS) void cross_attn_sum_kernel(const float* part, int n, long count, T* to) {
+    const long i = (long)blockIdx.x * CA_THREADS + threadIdx.x;
+    if (i >= count) return;
+    f32x4 y = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) y += *(const f32x4*)(part + (s * count + i) * 4);
+    put<T>(nullptr, to + i * 4, y);
+}
+
 // ---- backward: dq -----------------------------------------------------------------------------------------------------------
 // The forward's shape: one row per lane; q and do stay in registers, every key tile is read once per row tile.
 // Both sides of the backward together form seven products where one with atomics would form five: the price of sums of a fixed order.  Bound like the
@@ -529,10 +552,11 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
     const LdsTile<T, DP, BK> sK{(typename Term<T>::E*)smem}, sV{(typename Term<T>::E*)(smem + G::bytes(BK))};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wq = wave / NWK, wk = wave % NWK, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (R + 32 * NWQ - 1) / (32 * NWQ);
-    const Work w = work_of(a, block, ntiles);
+    const Work w = work_of(a, block, ntiles * a.nq);
     if (!w.any) return;
-    const int tile = w.i, b = w.b, kvh = w.kvh;
-    const int end = length_of(a, b);
+    const int tile = w.i % ntiles, split = w.i / ntiles, b = w.b, kvh = w.kvh;
+    const Range keys = range_of(length_of(a, b), a.nq, split);
+    const int begin = keys.begin, end = keys.end;
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const T* k = (const T*)a.k + b * a.k_b + kvh * a.k_h;
     const T* v = (const T*)a.v + b * a.v_b + kvh * a.v_h;
@@ -541,9 +565,9 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
     const long out_row = ((long)b * a.U + u) * a.H + kvh * share + g;
 
     RowTile<T, DP, BK> tk, tv;
-    if (end > 0) {
-        tk.load(k, a.k_t, end, a.D, tid);
-        tv.load(v, a.v_t, end, a.D, tid);
+    if (begin < end) {
+        tk.load(k + (long)begin * a.k_t, a.k_t, end - begin, a.D, tid);
+        tv.load(v + (long)begin * a.v_t, a.v_t, end - begin, a.D, tid);
     }
     Frag<T> qf[G::NCH], dof[G::NCH];
     float delta = 0.f;
@@ -565,7 +589,7 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
 
-    for (int k0 = 0; k0 < end; k0 += BK) {
+    for (int k0 = begin; k0 < end; k0 += BK) {
         __syncthreads();
         tk.store(sK, tid);
         tv.store(sV, tid);
@@ -619,14 +643,14 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
     }
     if (!live) return;
     T* o = (T*)a.dq + out_row * a.D;
+    float* part = a.part_q + ((long)split * a.B * a.U * a.H + out_row) * a.D;
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int d = i * 32 + 8 * x + 4 * h;
-            using V4 = __attribute__((ext_vector_type(4))) T;
             const f32x4 y = {acc[i][4 * x] * a.scale, acc[i][4 * x + 1] * a.scale, acc[i][4 * x + 2] * a.scale, acc[i][4 * x + 3] * a.scale};
-            if (d < a.D) *(V4*)(o + d) = __builtin_convertvector(y, V4);
+            if (d < a.D) put(a.nq > 1 ? part + d : nullptr, o + d, y);
         }
 }
 
@@ -648,10 +672,12 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
     float* sD = sL + BR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave / NWR, wr = wave % NWR, h = lane >> 5;
     const int share = a.H / a.Hkv, R = a.U * share, ntiles = (a.T + 32 * NWK - 1) / (32 * NWK);
-    const Work w = work_of<32 * NWK>(a, block, ntiles);
+    const Work w = work_of<32 * NWK>(a, block, ntiles * a.nk);
     if (!w.any) return;
-    const int tile = w.i, b = w.b, kvh = w.kvh;
+    const int tile = w.i % ntiles, split = w.i / ntiles, b = w.b, kvh = w.kvh;
     const int len = length_of(a, b);
+    const Range rows = range_of(R, a.nk, split);
+    const int first = rows.begin, last = rows.end;
     const T* q = (const T*)a.q + b * a.q_b + (long)kvh * share * a.q_h;
     const long row_base = (long)b * a.U * a.H + kvh * share;
     const T *dout = (const T*)a.dout + row_base * a.D, *out = (const T*)a.o + row_base * a.D;
@@ -664,14 +690,14 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
     if (any) {
         constexpr int P = pow2_from(G::CPR);
         RowTile<T, DP, BR, P> tq, to, ty;
-        RowWalk<G::EL, BR, P> at(a.q_u, a.q_h, (long)a.H * a.D, a.D, share, tid);
-        RowWalk<1, BR, 1> ls(0, 0, a.H, 1, share, tid);         // (one row per thread)
+        RowWalk<G::EL, BR, P> at(a.q_u, a.q_h, (long)a.H * a.D, a.D, share, first, tid);
+        RowWalk<1, BR, 1> ls(0, 0, a.H, 1, share, first, tid);         // (one row per thread)
         float rl = INFINITY;
         auto fetch = [&]() {
-            tq.load(q, at.a, at, R, a.D);
-            to.load(dout, at.b, at, R, a.D);
-            ty.load(out, at.b, at, R, a.D);
-            rl = ls.inside(0, R, 1) ? a.lse[row_base + ls.b[0]] - P_SHIFT<T> : INFINITY;      // rows behind the last: p = exp2(s - inf) = 0
+            tq.load(q, at.a, at, last, a.D);
+            to.load(dout, at.b, at, last, a.D);
+            ty.load(out, at.b, at, last, a.D);
+            rl = ls.inside(0, last, 1) ? a.lse[row_base + ls.b[0]] - P_SHIFT<T> : INFINITY;      // rows behind the last: p = exp2(s - inf) = 0
             at.next();
             ls.next();
         };
@@ -687,7 +713,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
                 vf[c] = frag_at((const T*)a.v + b * a.v_b + kvh * a.v_h + (long)key * a.v_t, c * 16 + h * 8, a.D);
             }
         }
-        for (int r0 = 0; r0 < R; r0 += BR) {
+        for (int r0 = first; r0 < last; r0 += BR) {
             if (!EARLY) fetch();
             __syncthreads();
             tq.store(sQ, tid);
@@ -695,11 +721,11 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
             to.products(ty, P_BACK, sD, tid);
             if (tid < BR) sL[tid] = rl;
             __syncthreads();
-            if (EARLY && r0 + BR < R) fetch();
+            if (EARLY && r0 + BR < last) fetch();
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int x0 = (wr * RT + t) * 32;
-                if (r0 + x0 >= R) continue;
+                if (r0 + x0 >= last) continue;
                 f32x16 s = f32x16{0}, dp = f32x16{0};
 #pragma unroll
                 for (int c = 0; c < G::NCH; ++c) {
@@ -755,20 +781,19 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
         if (wr != 0) return;
     }
     if (key >= a.T) return;
-    const float f = key < len ? 1.f : 0.f;
-    const long at = (((long)b * a.T + key) * a.Hkv + kvh) * a.D;
+    const long at = (((long)b * a.T + key) * a.Hkv + kvh) * a.D, all = (long)a.B * a.T * a.Hkv * a.D;
+    float* part = a.part_k + split * all + at;
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int d = i * 32 + 8 * x + 4 * h;
-            using V4 = __attribute__((ext_vector_type(4))) T;
             f32x4 y = {dk[i][4 * x], dk[i][4 * x + 1], dk[i][4 * x + 2], dk[i][4 * x + 3]};
             f32x4 z = {dv[i][4 * x], dv[i][4 * x + 1], dv[i][4 * x + 2], dv[i][4 * x + 3]};
-            if (f == 0.f) y = z = f32x4{0, 0, 0, 0};     // (a masked key's lane held whatever the zeroed operands gave)
+            if (key >= len) y = z = f32x4{0, 0, 0, 0};     // (a masked key's lane held whatever the zeroed operands gave)
             if (d < a.D) {
-                *(V4*)((T*)a.dk + at + d) = __builtin_convertvector(y * a.scale, V4);
-                *(V4*)((T*)a.dv + at + d) = __builtin_convertvector(z * P_BACK, V4);
+                put(a.nk > 1 ? part + d : nullptr, (T*)a.dk + at + d, y * a.scale);
+                put(a.nk > 1 ? part + a.nk * all + d : nullptr, (T*)a.dv + at + d, z * P_BACK);
             }
         }
 }
@@ -822,22 +847,41 @@ template <class T, int DP> int fwd_dp(const CrossAttnArgs& a, hipStream_t stream
     return launch(cross_attn_join_kernel<T>, (items + CA_THREADS - 1) / CA_THREADS, a, stream);
 }
 
-// Backward (a side whose gradients nobody wants is left out): both sides wide where that makes two workgroups per CU, fp32 one (its narrow shape has a CU to itself too: 41 against 56 us at 32 x 128
+// Backward: both sides wide where that makes two workgroups per CU, fp32 one (its narrow shape has a CU to itself too: 41 against 56 us at 32 x 128
 // over 100 heads of 128; not where most of 128 rows would be empty), else both narrow.
+bool bwd_wide(int B, int U, int T, int H, int Hkv, bool fp32) {
+    const long R = (long)U * (H / Hkv), n = (long)B * Hkv * ((R + 127) / 128 + (T + 127) / 128);
+    return n >= 2 * CA_CUS || (fp32 && R > 64 && n >= CA_CUS);
+}
+
+// (a side whose gradients nobody wants is left out)
 template <class T, int DP> int bwd_dp(const CrossAttnArgs& args, hipStream_t stream) {
     CrossAttnArgs a = args;
-    const long R = (long)a.U * (a.H / a.Hkv), bh = (long)a.B * a.Hkv;
-    const long n = bh * ((R + 127) / 128 + (a.T + 127) / 128);
-    const bool wide = n >= 2 * CA_CUS || (sizeof(T) == 4 && R > 64 && n >= CA_CUS);
-    const long per = wide ? 128 : 64, rows = a.dq ? blocks_of(a, (R + per - 1) / per) : 0, keys = a.dk ? blocks_of(a, (a.T + per - 1) / per) : 0;
+    const long R = (long)a.U * (a.H / a.Hkv);
+    const bool wide = bwd_wide(a.B, a.U, a.T, a.H, a.Hkv, sizeof(T) == 4);
+    const long per = wide ? 128 : 64, rows = a.dq ? blocks_of(a, a.nq * ((R + per - 1) / per)) : 0, keys = a.dk ? blocks_of(a, a.nk * ((a.T + per - 1) / per)) : 0;
     if (rows + keys == 0) return LAS_OK;
     LAS_TRY(check_grid(rows + keys));
     a.longest_first = a.lens && a.B > 1 && a.B <= 64 && rows + keys > 2 * CA_CUS;
     // (a workgroup of the key side goes over the rows in 16 products a tile, one of the row side over the keys in 12)
-    const int keys_first = R * 4 >= (long)a.T * 3, first = (int)(keys_first ? keys : rows);
+    const int keys_first = R / a.nk * 4 >= a.T / a.nq * 3, first = (int)(keys_first ? keys : rows);
     if (wide) hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 4, DEEP_BWD<T, DP>>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
     else hipLaunchKernelGGL((cross_attn_bwd_kernel<T, DP, 2, 1>), dim3((unsigned)(rows + keys)), dim3(CA_THREADS), 0, stream, a, first, keys_first);
     LAS_LAUNCH_CHECK();
+    const long nr = (long)a.B * a.U * a.H * a.D / 4, nkv = (long)a.B * a.T * a.Hkv * a.D / 4;
+    auto sum = [&](const float* part, int n, long count, void* to) -> int {
+        const long grid = (count + CA_THREADS - 1) / CA_THREADS;
+        if (grid == 0) return LAS_OK;
+        LAS_TRY(check_grid(grid));
+        hipLaunchKernelGGL(cross_attn_sum_kernel<T>, dim3((unsigned)grid), dim3(CA_THREADS), 0, stream, part, n, count, (T*)to);
+        LAS_LAUNCH_CHECK();
+        return LAS_OK;
+    };
+    if (a.dq && a.nq > 1) LAS_TRY(sum(a.part_q, a.nq, nr, a.dq));
+    if (a.dk && a.nk > 1) {
+        LAS_TRY(sum(a.part_k, a.nk, nkv, a.dk));
+        LAS_TRY(sum(a.part_k + (long)a.nk * nkv * 4, a.nk, nkv, a.dv));
+    }
     return LAS_OK;
 }
 
@@ -858,6 +902,20 @@ int cross_attn_splits(int B, int U, int T, int H, int Hkv, int dtype) {
     const long R = (long)U * (H / Hkv), per = fwd_wide(B, U, T, H, Hkv) ? 128 : 32, wgs = (long)B * Hkv * ((R + per - 1) / per);
     const long want = wgs >= CA_CUS ? 1 : 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / (dtype == 0 ? 128 : per == 128 ? 512 : 256);
     return (int)(want < 2 || most < 2 ? 1 : (want < most ? want : most));
+}
+
+// Ranges of a backward side that has few workgroups of long loops: of the keys for a few rows, of the rows for a few keys; as many as give every CU a
+// workgroup, none shorter than 256 (128 of fp32), where that side has at most half a workgroup per CU, the key side, which has twice the partial sums, a
+// quarter.  A range costs its partial sum in fp32 and the launches that add them up.  (16-bit heads of 64: 8 heads of 20 rows over 20000, 451 -> 38 us; 8 heads
+// of 2000 rows on one over 50, 360 -> 58; 4 x 100 over 3000, 77 -> 36, fp32 201 -> 84.  8 x 300 rows on 2 heads of 128 over 1700, 108 key workgroups, 169 against 178.)
+void cross_attn_bwd_splits(int B, int U, int T, int H, int Hkv, int dtype, int& nq, int& nk) {
+    const long R = (long)U * (H / Hkv), bh = (long)B * Hkv, per = bwd_wide(B, U, T, H, Hkv, dtype == 0) ? 128 : 64;
+    auto ranges = [&](long tiles, long length, int few) {
+        const long wgs = bh * tiles, most = length / (dtype == 0 ? 128 : 256), want = wgs <= 0 || wgs > few ? 1 : CA_CUS / wgs;
+        return (int)(want < 2 || most < 2 ? 1 : want < most ? want : most);
+    };
+    nq = ranges((R + per - 1) / per, T, CA_CUS / 2);
+    nk = ranges((T + per - 1) / per, R, CA_CUS / 4);
 }
 
 int cross_attn(const CrossAttnArgs& a, int dtype, bool bwd, hipStream_t stream) {

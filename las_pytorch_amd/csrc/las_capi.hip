@@ -1509,8 +1509,16 @@ int las_cross_attention_fwd(const las_cross_attention_desc* d, const void* q, co
     return cross_attn(a, d->dtype, false, (hipStream_t)stream);
 }
 
+size_t las_cross_attention_bwd_workspace_floats(const las_cross_attention_desc* d) {
+    if (!d || d->B <= 0 || d->U < 0 || d->T < 0 || d->H <= 0 || d->Hkv <= 0 || d->D <= 0) return 0;
+    int nq, nk;
+    cross_attn_bwd_splits(d->B, d->U, d->T, d->H, d->Hkv, d->dtype, nq, nk);
+    const size_t rows = (size_t)d->B * d->U * d->H * d->D, keys = (size_t)d->B * d->T * d->Hkv * d->D;
+    return (nq > 1 ? nq * rows : 0) + (nk > 1 ? 2 * nk * keys : 0);
+}
+
 int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* key_lengths,
-                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* stream) {
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, float* workspace, void* stream) {
     LAS_TRY(cross_attention_check(d, q, k, v));
     if (d->B == 0) return LAS_OK;
     const bool rows = d->U > 0, keys = d->T > 0;
@@ -1519,6 +1527,10 @@ int las_cross_attention_bwd(const las_cross_attention_desc* d, const void* q, co
     LAS_REQUIRE((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "cross attention tensors: 16-byte aligned");
     CrossAttnArgs a = cross_attention_args(d, q, k, v, key_lengths);
     a.o = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+    cross_attn_bwd_splits(d->B, d->U, d->T, d->H, d->Hkv, d->dtype, a.nq, a.nk);
+    LAS_REQUIRE((a.nq == 1 && a.nk == 1) || (workspace && ((uintptr_t)workspace & 15) == 0), "cross attention workspace");
+    a.part_q = workspace;
+    if (a.nk > 1) a.part_k = workspace + (a.nq > 1 ? (size_t)a.nq * d->B * d->U * d->H * d->D : 0);
     return cross_attn(a, d->dtype, true, (hipStream_t)stream);
 }
 

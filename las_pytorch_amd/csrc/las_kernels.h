@@ -367,9 +367,12 @@ struct CrossAttnArgs {
     const int* lens;               // valid frames per utterance (clamped to [0, T]); NULL: all
     long q_b, q_u, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
     int B, U, T, H, Hkv, D, nsplit, longest_first;
+    int nq, nk;                    // backward: ranges of the keys (row side), of the rows (key side)
+    float *part_q, *part_k;        // their partial sums: nq of dq; nk of dk, then nk of dv
     float scale, c;                // c = scale log2(e)
 };
 int cross_attn_splits(int B, int U, int T, int H, int Hkv, int dtype);
+void cross_attn_bwd_splits(int B, int U, int T, int H, int Hkv, int dtype, int& nq, int& nk);
 int cross_attn(const CrossAttnArgs& a, int dtype, bool bwd, hipStream_t stream);      // dtype 0 fp32, 1 bf16, 2 fp16
 
 // ---- distill.hip -----------------------------------------------------------------------

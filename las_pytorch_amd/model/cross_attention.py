@@ -55,7 +55,9 @@ def _lengths(key_lengths, B, T, device):
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_floats(B, U, T, H, Hkv, D, code):
-    return lib().las_cross_attention_workspace_floats(CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D, dtype=code))
+    """Of the forward, of the backward."""
+    d = CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D, dtype=code)
+    return lib().las_cross_attention_workspace_floats(d), lib().las_cross_attention_bwd_workspace_floats(d)
 
 
 def _forward(query, key, value, key_lengths, scale, want_lse):
@@ -77,20 +79,19 @@ def _forward(query, key, value, key_lengths, scale, want_lse):
     d = CrossAttentionDesc(B, U, T, H, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     out = torch.empty(qs, device=device, dtype=dtype)
     lse = torch.empty((B, U, H), device=device, dtype=torch.float32) if want_lse else None
-    n = _workspace_floats(B, U, T, H, Hkv, D, code)
+    n, n_bwd = _workspace_floats(B, U, T, H, Hkv, D, code)
     work = torch.empty(n, device=device, dtype=torch.float32) if n else None
     _cabi.call_on(device, lib().las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                   None if work is None else work.data_ptr())
-    return d, q, k, v, key_lengths, out, lse
+    return d, n_bwd, q, k, v, key_lengths, out, lse
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, key_lengths, scale):
-        d, *saved = _forward(query, key, value, key_lengths, scale, True)
+        ctx.desc, ctx.work, *saved = _forward(query, key, value, key_lengths, scale, True)
         ctx.save_for_backward(*saved)
-        ctx.desc = d
         return saved[4]
 
     @staticmethod
@@ -106,9 +107,11 @@ class _CrossAttentionFn(torch.autograd.Function):
         if need_k or need_v:
             dk = torch.empty_like(k, memory_format=torch.contiguous_format)
             dv = torch.empty_like(dk)
+        work = torch.empty(ctx.work, device=device, dtype=torch.float32) if ctx.work else None
         _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                      None if dq is None else dq.data_ptr(), None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr())
+                      None if dq is None else dq.data_ptr(), None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
+                      None if work is None else work.data_ptr())
         return dq, dk, dv, None, None
 
 
@@ -128,4 +131,4 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
             raise RuntimeError(f"cross_attention: scale must be positive, got {scale}")
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _CrossAttentionFn.apply(query, key, value, key_lengths, scale)
-    return _forward(query, key, value, key_lengths, scale, False)[5]
+    return _forward(query, key, value, key_lengths, scale, False)[6]

@@ -123,6 +123,10 @@ SHAPES = [  # B, U, T, H, Hkv, D
     (2, 150, 1500, 4, 2, 64),      # 128 rows and key ranges
     (1, 100, 1100, 2, 2, 128),
     (2, 9, 300, 4, 4, 96),         # key ranges of fp32 alone
+    (2, 700, 40, 4, 2, 64),        # row ranges in the backward
+    (1, 1100, 70, 6, 2, 128),
+    (3, 4, 1103, 4, 2, 128),       # key ranges in the backward
+    (1, 600, 600, 2, 1, 32),       # both
 ]
 
 
@@ -338,7 +342,7 @@ def test_c_entry_refuses_before_it_launches():
                    dict(U=1 << 30), dict(T=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf)):
         d = _cabi.CrossAttentionDesc(**{**good, **change})
         assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, 4096, None, None, None) == 1, change
-        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, None) == 1, change
+        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, 4096, None) == 1, change
         assert b"cross attention" in L.las_last_error()
     d = _cabi.CrossAttentionDesc(**good)
     for at in range(3):
@@ -348,12 +352,18 @@ def test_c_entry_refuses_before_it_launches():
         ptrs[at] = 4100
         assert L.las_cross_attention_fwd(d, *ptrs, None, 4096, None, None, None) == 1
     assert L.las_cross_attention_fwd(d, 4096, 4096, 4096, None, None, None, None, None) == 1
-    assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, None, 4096, 4096, 4096, 4096, None) == 1
+    assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, None, 4096, 4096, 4096, 4096, None, None) == 1
     for grads in ((None, 4096, None), (4096, None, 4096), (None, None, None)):       # half of a side, nothing at all
-        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, *grads, None) == 1
+        assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, *grads, None, None) == 1
     assert L.las_cross_attention_fwd(None, 4096, 4096, 4096, None, 4096, None, None, None) == 1
     assert L.las_cross_attention_workspace_floats(d) == 0
     assert L.las_cross_attention_workspace_floats(_cabi.CrossAttentionDesc(**{**good, "T": 4096})) > 0
+    assert L.las_cross_attention_bwd_workspace_floats(d) == 0
+    for long in (dict(T=4096), dict(U=4096)):        # a few rows over many keys, many rows over a few keys: partial sums want a workspace
+        d = _cabi.CrossAttentionDesc(**{**good, **long})
+        assert L.las_cross_attention_bwd_workspace_floats(d) > 0
+        for workspace in (None, 4100):
+            assert L.las_cross_attention_bwd(d, 4096, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, workspace, None) == 1
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         cross_attention(*(torch.zeros(1, 2, 2, 32) for _ in range(3)))
     assert "cross_attention" in las_pytorch_amd.__all__
