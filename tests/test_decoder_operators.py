@@ -127,3 +127,53 @@ def test_two_streams_and_one_graph_of_all():
         for out in held:
             for a, b in zip(out, want):
                 assert torch.equal(a, b), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_saved_tensors_kept_elsewhere(dtype):
+    """Saved tensors that come back at another address (kept on the host) and forwards that are run again: the bits of the plain backward."""
+    from torch.utils.checkpoint import checkpoint
+
+    g = torch.Generator().manual_seed(12)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()      # noqa: E731
+    q, k, v, dout = r(3, 20, 4, 64), r(3, 200, 2, 64), r(3, 200, 2, 64), r(3, 20, 4, 64)
+    frames = torch.tensor([200, 0, 77], device="cuda")
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    want = torch.autograd.grad(cross_attention(*leaves, frames), leaves, dout)
+    with torch.autograd.graph.save_on_cpu():
+        out = cross_attention(*leaves, frames)
+    again = checkpoint(lambda *x: cross_attention(*x, frames), *leaves, use_reentrant=False)
+    for o in (out, again):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(o, leaves, dout), want))
+
+    index, teacher, steps = torch.randint(0, 700, (3, 5, 6), generator=g).cuda(), r(3, 5, 6), torch.tensor([5, 0, 3], device="cuda")
+    for z in (r(3, 5, 700), r(5, 3, 700).transpose(0, 1)):
+        z = z.detach().requires_grad_(True)
+        (want,) = torch.autograd.grad(S.distillation_loss_device(z, index, teacher, 2.0, steps), (z,))
+        with torch.autograd.graph.save_on_cpu():
+            loss = S.distillation_loss_device(z, index, teacher, 2.0, steps)
+        for keep in (True, False):
+            (got,) = torch.autograd.grad(loss, (z,), retain_graph=keep)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_one_tensor_in_several_places():
+    """Keys that are the values and the queries too, and a student whose rows are one: gradients of the shared tensor are the sums."""
+    g = torch.Generator().manual_seed(13)
+    x, dout = torch.randn(2, 40, 4, 64, generator=g).cuda(), torch.randn(2, 40, 4, 64, generator=g).cuda()
+    apart = [x.clone().requires_grad_(True) for _ in range(3)]
+    want = torch.autograd.grad(cross_attention(*apart), apart, dout)
+    x.requires_grad_(True)
+    out = cross_attention(x, x, x)
+    (got,) = torch.autograd.grad(out, (x,), dout)
+    assert torch.equal(out, cross_attention(*apart))
+    assert ((got - sum(want)).abs() <= 2 * 2.0 ** -24 * sum(w.abs() for w in want)).all()       # (two additions, in any order)
+
+    row = torch.randn(1, 1, 300, generator=g).cuda().requires_grad_(True)
+    index, teacher = torch.randint(0, 300, (3, 4, 5), generator=g).cuda(), torch.randn(3, 4, 5, generator=g).cuda()
+    apart = row.detach().expand(3, 4, 300).contiguous().requires_grad_(True)
+    (want,) = torch.autograd.grad(S.distillation_loss_device(apart, index, teacher), (apart,))
+    (got,) = torch.autograd.grad(S.distillation_loss_device(row.expand(3, 4, 300), index, teacher), (row,))
+    assert ((got - want.sum((0, 1), keepdim=True)).abs() <= 24 * 2.0 ** -24 * want.abs().sum((0, 1), keepdim=True)).all()     # (twelve terms, both ways)
