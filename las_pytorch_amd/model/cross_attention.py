@@ -11,14 +11,6 @@ from .. import _cabi
 from .._cabi import DTYPES, CrossAttentionDesc, lib
 
 
-def _rows(t, per16):
-    """``t`` itself when its rows (last dimension) are contiguous and start at multiples of 16 bytes, else a contiguous copy."""
-    sb, st, sh, sd = t.stride()
-    if sd == 1 and not (sb | st | sh) % per16 and not t.data_ptr() & 15:
-        return t
-    return _aligned(t.contiguous())
-
-
 def _aligned(t):
     return t if not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
@@ -54,37 +46,53 @@ def _lengths(key_lengths, B, T, device):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_floats(B, U, T, H, Hkv, D, code):
-    """Of the forward, of the backward."""
-    d = CrossAttentionDesc(B=B, U=U, T=T, H=H, Hkv=Hkv, D=D, dtype=code)
-    return lib().las_cross_attention_workspace_floats(d), lib().las_cross_attention_bwd_workspace_floats(d)
-
-
-def _forward(query, key, value, key_lengths, scale, want_lse):
-    dtype = query.dtype
-    qs, ks = query.shape, key.shape
+def _plan(qs, ks, vs, q_strides, k_strides, v_strides, dtype, scale):
+    """What a call's shapes and strides settle, so that a decode loop settles it once: whether they go together at all, which operands have to be
+    copied to contiguous rows, the library's descriptor, and the workspaces of the forward and the backward.  (Read by the library, never written.)"""
     code = DTYPES.get(dtype)
-    if (code is None or len(qs) != 4 or len(ks) != 4 or ks != value.shape or not query.is_cuda or key.dtype != dtype or value.dtype != dtype
-            or key.device != query.device or value.device != query.device):
-        _refuse(query, key, value)
+    if code is None or len(qs) != 4 or len(ks) != 4 or ks != vs:
+        return None
     B, U, H, D = qs
     T, Hkv = ks[1], ks[2]
     per16 = 4 if code == 0 else 8
     if ks[0] != B or ks[3] != D or Hkv < 1 or H < 1 or H % Hkv or not 0 < D <= 128 or D % per16:
+        return None
+    copied, strides = [], []
+    for shape, (sb, st, sh, sd) in ((qs, q_strides), (ks, k_strides), (ks, v_strides)):
+        fits = sd == 1 and not (sb | st | sh) % per16
+        copied.append(not fits)
+        strides += (sb, st, sh) if fits else (shape[1] * shape[2] * D, shape[2] * D, D)
+    d = CrossAttentionDesc(B, U, T, H, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, *strides)
+    return d, copied, lib().las_cross_attention_workspace_floats(d), lib().las_cross_attention_bwd_workspace_floats(d)
+
+
+def _forward(query, key, value, key_lengths, scale, want_lse):
+    device, dtype, qs, ks = query.device, query.dtype, query.shape, key.shape
+    plan = _plan(qs, ks, value.shape, query.stride(), key.stride(), value.stride(), dtype, scale)
+    if plan is None or not query.is_cuda or key.dtype != dtype or value.dtype != dtype or key.device != device or value.device != device:
         _refuse(query, key, value)
-    device = query.device
+    d, copied, n, n_bwd = plan
     if key_lengths is not None:
-        key_lengths = _lengths(key_lengths, B, T, device)
-    q, k, v = _rows(query, per16), _rows(key, per16), _rows(value, per16)
-    d = CrossAttentionDesc(B, U, T, H, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        key_lengths = _lengths(key_lengths, qs[0], ks[1], device)
+    q, k, v = query, key, value
+    if True in copied:
+        q, k, v = (x.contiguous() if c else x for x, c in zip((q, k, v), copied))
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        d, q, k, v = _realigned(d, q, k, v)
     out = torch.empty(qs, device=device, dtype=dtype)
-    lse = torch.empty((B, U, H), device=device, dtype=torch.float32) if want_lse else None
-    n, n_bwd = _workspace_floats(B, U, T, H, Hkv, D, code)
+    lse = torch.empty(qs[:3], device=device, dtype=torch.float32) if want_lse else None
     work = torch.empty(n, device=device, dtype=torch.float32) if n else None
     _cabi.call_on(device, lib().las_cross_attention_fwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                   None if work is None else work.data_ptr())
     return d, n_bwd, q, k, v, key_lengths, out, lse
+
+
+def _realigned(d, q, k, v):
+    """Operands that start between 16-byte pieces, copied."""
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    return CrossAttentionDesc(d.B, d.U, d.T, d.H, d.Hkv, d.D, d.dtype, d.scale, *strides), q, k, v
 
 
 class _CrossAttentionFn(torch.autograd.Function):
