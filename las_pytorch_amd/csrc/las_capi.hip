@@ -1403,7 +1403,7 @@ static int distill_call(const las_distill_desc* d, const void* logits, const voi
     LAS_REQUIRE(d->dtype >= 0 && d->dtype <= 2 && d->teacher_dtype >= 0 && d->teacher_dtype <= 2, "distillation dtype");
     LAS_REQUIRE(d->B > 0 && d->U > 0 && d->V > 0 && d->V < (1 << 30) && d->K > 0 && d->K <= 1024 && (int64_t)d->B * d->U < 0x7fffffffLL,
                 "distillation dims (1 <= K <= 1024)");
-    LAS_REQUIRE(d->temperature > 0.f && d->temperature < 1e30f, "distillation temperature: positive");
+    LAS_REQUIRE(d->temperature > 1e-30f && d->temperature < 1e30f, "distillation temperature: positive (1e-30 to 1e30)");
     LAS_REQUIRE(loss || dlogits, "distillation outputs");
     LAS_REQUIRE(!loss || scratch, "distillation scratch");
     LAS_REQUIRE(!unless_one || upstream, "distillation factor");

@@ -249,8 +249,8 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     if teacher_logits.requires_grad:
         raise RuntimeError("distillation_loss_device has no gradient for the teacher: detach teacher_logits")
     temperature = float(temperature)
-    if not 0.0 < temperature < 1e30:
-        raise RuntimeError(f"distillation_loss_device: temperature must be positive, got {temperature}")
+    if not 1e-30 < temperature < 1e30:       # (its reciprocal is an fp32 factor)
+        raise RuntimeError(f"distillation_loss_device: temperature must be positive (1e-30 to 1e30), got {temperature}")
     if not 1 <= teacher_index.shape[2] <= 1024 or pred_y.numel() == 0:
         raise RuntimeError("distillation_loss_device: between 1 and 1024 teacher entries per row and at least one row are needed")
     if lengths is not None:

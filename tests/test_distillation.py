@@ -296,7 +296,7 @@ def test_c_entry_refuses_before_it_launches():
     names = ["logits", "index", "teacher", "lengths", "loss", "dlogits", "upstream", "scratch", "stream"]
     good = dict(logits=4096, index=4096, teacher=4096, lengths=None, loss=4096, dlogits=4096, upstream=4096, scratch=4096, stream=None)
     for change in (dict(dtype=3), dict(dtype=-1), dict(teacher_dtype=3), dict(B=0), dict(U=0), dict(V=0), dict(V=1 << 30), dict(K=0), dict(K=1025),
-                   dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(B=1 << 20, U=1 << 20)):
+                   dict(temperature=0.0), dict(temperature=1e-35), dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(B=1 << 20, U=1 << 20)):
         d = _cabi.DistillDesc(**{**shape, **change})
         assert L.las_distill_loss(d, *(good[n] for n in names)) == 1, change
         assert L.las_distill_grad_unless_one(d, *(good[n] for n in names if n not in ("loss", "scratch"))) == 1, change
