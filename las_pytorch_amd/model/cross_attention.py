@@ -74,11 +74,7 @@ def _forward(query, key, value, key_lengths, scale, want_lse):
     d, copied, n, n_bwd = plan
     if key_lengths is not None:
         key_lengths = _lengths(key_lengths, qs[0], ks[1], device)
-    q, k, v = query, key, value
-    if True in copied:
-        q, k, v = (x.contiguous() if c else x for x, c in zip((q, k, v), copied))
-    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
-        d, q, k, v = _realigned(d, q, k, v)
+    d, q, k, v = _addressed(d, copied, query, key, value)
     out = torch.empty(qs, device=device, dtype=dtype)
     lse = torch.empty(qs[:3], device=device, dtype=torch.float32) if want_lse else None
     work = torch.empty(n, device=device, dtype=torch.float32) if n else None
@@ -88,11 +84,16 @@ def _forward(query, key, value, key_lengths, scale, want_lse):
     return d, n_bwd, q, k, v, key_lengths, out, lse
 
 
-def _realigned(d, q, k, v):
-    """Operands that start between 16-byte pieces, copied."""
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    return CrossAttentionDesc(d.B, d.U, d.T, d.H, d.Hkv, d.D, d.dtype, d.scale, *strides), q, k, v
+def _addressed(d, copied, q, k, v):
+    """Operands whose rows the library can address, and the descriptor of them: what the plan says has to be copied is copied, as is what starts
+    between 16-byte pieces."""
+    if True in copied:
+        q, k, v = (x.contiguous() if c else x for x, c in zip((q, k, v), copied))
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        d = CrossAttentionDesc(d.B, d.U, d.T, d.H, d.Hkv, d.D, d.dtype, d.scale, *strides)
+    return d, q, k, v
 
 
 class _CrossAttentionFn(torch.autograd.Function):
@@ -100,14 +101,20 @@ class _CrossAttentionFn(torch.autograd.Function):
     def forward(ctx, query, key, value, key_lengths, scale):
         ctx.desc, ctx.work, *saved = _forward(query, key, value, key_lengths, scale, True)
         ctx.save_for_backward(*saved)
+        ctx.scale, ctx.strides = scale, [x.stride() for x in saved[:3]]
         return saved[4]
 
     @staticmethod
     @_cabi.differentiable_once
     def backward(ctx, dout):
         q, k, v, key_lengths, out, lse = ctx.saved_tensors
-        dout = _aligned(dout.contiguous())
-        device = q.device
+        d, device = ctx.desc, q.device
+        dout, out, lse = _aligned(dout.contiguous()), _aligned(out.contiguous()), lse.contiguous()
+        if key_lengths is not None:
+            key_lengths = key_lengths.contiguous()
+        # saved tensors may have been elsewhere in between (hooks that keep them on the host, say) and come back in another layout
+        if [q.stride(), k.stride(), v.stride()] != ctx.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+            d, q, k, v = _addressed(*_plan(q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, ctx.scale)[:2], q, k, v)
         dq = dk = dv = None
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         if need_q:
@@ -116,7 +123,7 @@ class _CrossAttentionFn(torch.autograd.Function):
             dk = torch.empty_like(k, memory_format=torch.contiguous_format)
             dv = torch.empty_like(dk)
         work = torch.empty(ctx.work, device=device, dtype=torch.float32) if ctx.work else None
-        _cabi.call_on(device, lib().las_cross_attention_bwd, ctx.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _cabi.call_on(device, lib().las_cross_attention_bwd, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       None if key_lengths is None else key_lengths.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                       None if dq is None else dq.data_ptr(), None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
                       None if work is None else work.data_ptr())
