@@ -190,6 +190,10 @@ class _DistillationLoss(torch.autograd.Function):
     @_cabi.differentiable_once
     def backward(ctx, upstream):
         logits, index, teacher, lengths = ctx.saved_tensors
+        # (hooks on saved tensors may have brought them back in another layout)
+        logits, index, teacher = logits if logits.stride(2) == 1 else logits.contiguous(), index.contiguous(), teacher.contiguous()
+        if lengths is not None:
+            lengths = lengths.contiguous()
         lens = None if lengths is None else lengths.data_ptr()
         grad = None
         if not torch.cuda.is_current_stream_capturing() and logits.stride() == ctx.strides:

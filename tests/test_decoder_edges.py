@@ -5,6 +5,7 @@ import torch
 
 from las_pytorch_amd import _cabi, cross_attention
 from las_pytorch_amd.model import cross_attention as ca
+from las_pytorch_amd.solver import solver as S
 
 
 class Recorder:
@@ -13,6 +14,7 @@ class Recorder:
     def __init__(self, monkeypatch):
         self.calls = []
         monkeypatch.setattr(ca, "_refuse", lambda *operands: None)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
         monkeypatch.setattr(_cabi, "call_on", lambda device, fn, *args: self.calls.append(args))
 
 
@@ -38,6 +40,21 @@ def _views(dtype, device, seed=31):
             "plain": (r(B, U, H, D), r(B, T, Hkv, D), r(B, T, Hkv, D))}
 
 
+def _keep_all(monkeypatch, alive):
+    """Every tensor that .contiguous() or .clone() gives stays alive (what is freed could come back at the address of another)."""
+    keep = lambda f: lambda x, *a, **k: (alive.append(f(x, *a, **k)), alive[-1])[1]      # noqa: E731
+    monkeypatch.setattr(torch.Tensor, "contiguous", keep(torch.Tensor.contiguous))
+    monkeypatch.setattr(torch.Tensor, "clone", keep(torch.Tensor.clone))
+
+
+def _held_at(address, like, strides, alive):
+    """The values that a kernel reads at ``address`` by ``strides``, none of them outside the storage that lies there."""
+    (held,) = {id(x): x for x in alive if x.data_ptr() == address and x.shape == like.shape}.values()
+    last = held.storage_offset() + sum((n - 1) * s for n, s in zip(like.shape, strides))
+    assert last < held.untyped_storage().nbytes() // held.element_size(), (strides, held.stride())
+    return held.as_strided(like.shape, strides)
+
+
 @pytest.mark.parametrize("how", ["dense", "permuted", "between"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("layout", ["fused", "time first", "heads first", "plain"])
@@ -46,13 +63,10 @@ def test_backward_addresses_the_tensors_that_arrive(monkeypatch, layout, dtype, 
     recorder = Recorder(monkeypatch)
     leaves = [x.detach().requires_grad_(True) for x in _views(dtype, "cpu")[layout]]
     lengths = torch.tensor([45, 0, 7], dtype=torch.int32)
-    alive = []                                          # (what is freed could come back at the address of another)
-    contiguous, clone = torch.Tensor.contiguous, torch.Tensor.clone
-    keep = lambda f: lambda x, *a, **k: (alive.append(f(x, *a, **k)), alive[-1])[1]      # noqa: E731
+    alive = []
     with torch.autograd.graph.saved_tensors_hooks(lambda x: _moved(x, how), lambda x: (alive.append(x), x)[1]):
         out = cross_attention(*leaves, lengths)
-    monkeypatch.setattr(torch.Tensor, "contiguous", keep(contiguous))
-    monkeypatch.setattr(torch.Tensor, "clone", keep(clone))
+    _keep_all(monkeypatch, alive)
     torch.autograd.grad(out, leaves, torch.ones_like(out))
     monkeypatch.undo()
     forward, backward = recorder.calls
@@ -61,13 +75,34 @@ def test_backward_addresses_the_tensors_that_arrive(monkeypatch, layout, dtype, 
     want = {0: (leaves[0], (d.q_b, d.q_u, d.q_h)), 1: (leaves[1], (d.k_b, d.k_t, d.k_h)), 2: (leaves[2], (d.v_b, d.v_t, d.v_h))}
     for i, (leaf, strides) in want.items():
         assert addresses[i] % 16 == 0
-        (held,) = {id(x): x for x in alive if x.data_ptr() == addresses[i] and x.shape == leaf.shape}.values()
-        last = held.storage_offset() + sum((n - 1) * s for n, s in zip(leaf.shape, (*strides, 1)))
-        assert last < held.untyped_storage().nbytes() // held.element_size(), (i, strides, held.stride())
-        assert torch.equal(held.as_strided(leaf.shape, (*strides, 1)), leaf), (i, strides, held.stride())
+        assert torch.equal(_held_at(addresses[i], leaf, (*strides, 1), alive), leaf), (i, strides)
     for i in (3, 4, 5):                                 # lengths, the output, its statistics: contiguous
         assert any(x.data_ptr() == addresses[i] and x.is_contiguous() for x in alive)
     assert addresses[4] % 16 == 0
+
+
+@pytest.mark.parametrize("how", ["dense", "permuted", "between"])
+@pytest.mark.parametrize("seed", [1.0, 2.0])
+@pytest.mark.parametrize("layout", ["plain", "step first", "padded"])
+def test_distillation_backward_addresses_the_tensors_that_arrive(monkeypatch, layout, seed, how):
+    """The same of the distillation loss, whose first backward hands over what the forward formed and whose second forms it anew."""
+    recorder = Recorder(monkeypatch)
+    g = torch.Generator().manual_seed(33)
+    r = lambda *s: torch.randn(*s, generator=g)      # noqa: E731
+    z = {"plain": r(3, 5, 40), "step first": r(5, 3, 40).transpose(0, 1), "padded": r(3, 5, 48)[..., :40]}[layout].requires_grad_(True)
+    index, teacher, lengths = torch.randint(0, 40, (3, 5, 4), generator=g), r(3, 5, 4), torch.tensor([5, 0, 2], dtype=torch.int32)
+    alive = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: _moved(x, how), lambda x: (alive.append(x), x)[1]):
+        loss = S._DistillationLoss.apply(z, index, teacher, lengths, 2.0)
+    _keep_all(monkeypatch, alive)
+    for keep in (True, False):
+        torch.autograd.grad(loss, (z,), torch.tensor(seed), retain_graph=keep)
+    monkeypatch.undo()
+    for d, *addresses in recorder.calls[1:]:
+        assert (d.B, d.U, d.V, d.K) == (3, 5, 40, 4)
+        assert torch.equal(_held_at(addresses[0], z, (d.stride_b, d.stride_u, 1), alive), z)
+        for at, like in zip(addresses[1:], (index, teacher, lengths)):
+            assert torch.equal(_held_at(at, like, torch.empty(like.shape).stride(), alive), like)
 
 
 @pytest.mark.gpu
