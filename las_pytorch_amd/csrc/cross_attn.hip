@@ -57,8 +57,9 @@ template <class T> static __device__ __forceinline__ f32x16 mma(f32x16 c, const 
     return mma16(c, a.p[0], b.p[0], E{});
 }
 
-// eight fp32 values as an operand.  16-bit types: rounding P and dS to the inputs' type costs half a step (2^-9 bf16, 2^-12 fp16) per term of sums
-// that stay in fp32.
+// eight fp32 values as an operand.  16-bit types: rounding P and dS to the inputs' type costs half a step (2^-8 bf16, 2^-11 fp16) per term of sums
+// that stay in fp32: the matrix instruction takes both operands in one type, and a second term would double the product.  (fp16 below its normal range: see
+// P_SHIFT and DS_SCALED.)
 template <class T> static __device__ __forceinline__ Frag<T> frag_of(f32x8 x) {
     using V8 = __attribute__((ext_vector_type(8))) typename Term<T>::E;
     Frag<T> f;
@@ -128,6 +129,42 @@ template <class T> constexpr float P_SHIFT_FWD = 0.f;
 template <> constexpr float P_SHIFT<_Float16> = 14.f;
 template <> constexpr float P_SHIFT_FWD<_Float16> = 9.f;
 constexpr float P_SLACK = 6.f;
+
+// dS has no such bound: it is as large as the output's gradient, which a mean over many rows makes small and a loss scale large.  In fp16 it is formed
+// f times its size, a power of two for each lane (a row in dq, a key in dk) that follows the largest dS of the lane's sum: it starts at 2^60, where what
+// is lost is below any fp16 result, and a tile that reaches beyond 2^15 takes it, and what was summed before, down to where that tile's largest lies between
+// 2^9 and 2^10.  What is rounded below fp16's normal range is then off by 2^-34 of the largest at most.  (Unscaled, a dS below 2^-25 is zero and one above
+// 65504 infinite.)  Price, a maximum per dS and on the key side a product: backward of 16 x 1024 over 2048, 16 on 4 heads of 32 277 -> 298 us, of 64 460 -> 465, of
+// 96 720 -> 750, of 128 933 -> 1026.
+template <class T> constexpr bool DS_SCALED = false;
+template <> constexpr bool DS_SCALED<_Float16> = true;
+template <class T> constexpr float DS_START = DS_SCALED<T> ? 0x1p60f : 1.f;
+// a tile's dS as it is formed and the sum so far: the power of two by which the scale changes
+template <class T, int NDT> static __device__ __forceinline__ int follow_ds(float& f, f32x16& ds, f32x16 (&acc)[NDT]) {
+    if constexpr (!DS_SCALED<T>) return 0;
+    float mx = fabsf(ds[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fabsf(ds[r]));
+    if (!__any(mx > 32768.f)) return 0;
+    mx = fmaxf(mx, __shfl_xor(mx, 32));         // (a lane's other half holds the rest of the same sum's terms, and the same scale)
+    const int by = mx > 32768.f ? min(10 - __builtin_amdgcn_frexp_expf(mx), 0) : 0;         // (an infinity has exponent 0 here, and stays one)
+    f = ldexpf(f, by);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] = ldexpf(ds[r], by);
+#pragma unroll
+    for (int i = 0; i < NDT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = ldexpf(acc[i][r], by);
+    return by;
+}
+template <class T, int NDT> static __device__ __forceinline__ void undo_ds(float f, f32x16 (&acc)[NDT]) {
+    if constexpr (!DS_SCALED<T>) return;
+    const int by = 1 - __builtin_amdgcn_frexp_expf(f);
+#pragma unroll
+    for (int i = 0; i < NDT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = ldexpf(acc[i][r], by);
+}
 
 // A tile of ROWS rows in LDS.
 template <class T, int DP, int ROWS> struct LdsTile {
@@ -625,6 +662,8 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
     }
     delta += other_half(delta);
     const float lse = live ? a.lse[out_row] : INFINITY;
+    float f = DS_START<T>;
+    delta *= f;
     f32x16 acc[G::NDT];
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i) acc[i] = f32x16{0};
@@ -649,12 +688,13 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
                 dp = mma<T>(dp, sV.row(r0 + (lane & 31), c, h), dof[c]);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse)) * (DS_SCALED<T> ? fmaf(dp[r], f, -delta) : dp[r] - delta);
             if (k0 + r0 + 32 > end) {            // (the keys behind the last: zeros in K, but exp2(-lse) need not be finite)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (k0 + r0 + 8 * (r >> 2) + 4 * h + (r & 3) >= end) s[r] = 0.f;
             }
+            delta = ldexpf(delta, follow_ds<T>(f, s, acc));
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const Frag<T> ds = pack<T>(s, c);
@@ -663,6 +703,7 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
             }
         }
     }
+    undo_ds<T>(f, acc);
     if constexpr (NWK > 1) {
         float* red = (float*)smem;
         __syncthreads();
@@ -753,6 +794,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
                 vf[c] = frag_at((const T*)a.v + b * a.v_b + kvh * a.v_h + (long)key * a.v_t, c * 16 + h * 8, a.D);
             }
         }
+        float f = DS_START<T>;
         for (int r0 = first; r0 < last; r0 += BR) {
             if (!EARLY) fetch();
             __syncthreads();
@@ -780,8 +822,10 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
                         const int r = 4 * x + e;
                         s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -ls[e]));
                         dp[r] = s[r] * fmaf(dp[r], P_BACK, -de[e]);
+                        if constexpr (DS_SCALED<T>) dp[r] *= f;
                     }
                 }
+                follow_ds<T>(f, dp, dk);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> p = pack<T>(s, c), ds = pack<T>(dp, c);
@@ -793,6 +837,7 @@ static __device__ __forceinline__ void cross_attn_dkv(const CrossAttnArgs& a, in
                 }
             }
         }
+        undo_ds<T>(f, dk);
     }
     if constexpr (NWR > 1) {
         if (any) {

@@ -1,5 +1,7 @@
 """Calls of the decoder operators at the edge of what their documentation allows: saved tensors that come back in another layout, sizes and types at
 the end of their range, derivatives that do not exist, gradients far from one."""
+import math
+
 import pytest
 import torch
 
@@ -119,3 +121,92 @@ def test_views_whose_saved_tensors_are_kept_on_the_host(layout, dtype, pinned):
         out = cross_attention(*leaves, lengths)
     for a, b in zip(torch.autograd.grad(out, leaves, dout), want):
         assert torch.equal(a, b)
+
+
+def half_precision_gradients(q, k, v, dout):
+    """Output and gradients of fp16 attention in 64 bits, each with the error that a kernel may have which keeps fp32 sums and rounds to fp16 the output, P, dS
+    and the results alone, dS relative to the largest that it is summed with:
+      P     half a step, 2^-11; P is formed 2^9 (forward) or 2^14 (backward) times too large, so a subnormal half step is 2^-34 or 2^-39 at most
+      dS    half a step, or half a subnormal step, 2^-25, at a scale where the largest of its sum is 2^9 at least: 2^-34 of that one (2^-33 here: the
+            largest has its own error)
+      rest  fp32: the scores (D + 4 roundings of the sum of absolute values, twice), the exponential (8), the statistic of up to log2 T (2 ln T), dO V and D
+            (D roundings; D from the rounded output), the sums over keys or rows (their length)
+      results and output: half a step, or half a subnormal step."""
+    h, f32, sub = 2.0 ** -11, 2.0 ** -24, 2.0 ** -25
+    B, U, H, D = q.shape
+    T, Hkv = k.shape[1:3]
+    scale, back = D ** -0.5, lambda x: x.permute(0, 2, 1, 3)      # noqa: E731
+    wide = lambda x: back(x.double()).repeat_interleave(H // Hkv, 1)      # noqa: E731
+    Q, K, V, dO = back(q.double()), wide(k), wide(v), back(dout.double())
+    rounded = lambda x: (h * x.abs()).clamp_min(sub) + f32 * x.abs()      # noqa: E731
+    P = torch.softmax(scale * Q @ K.transpose(2, 3), -1)
+    out = P @ V
+    rel = 2 * (D + 4) * f32 * (scale * Q.abs() @ K.abs().transpose(2, 3)).amax(-1, keepdim=True) + 8 * f32
+    E_out = rounded(out) + (h + rel + T * f32) * (P @ V.abs()) + 2.0 ** -34 * V.abs().sum(2, keepdim=True)
+    dp, delta = dO @ V.transpose(2, 3), (dO * out).sum(-1, keepdim=True)
+    ds = P * (dp - delta)
+    rel = rel + 2 * math.log(max(T, 2)) * f32
+    E_D = (dO.abs() * E_out).sum(-1, keepdim=True) + D * f32 * (dO * out).abs().sum(-1, keepdim=True)
+    E = P * (D * f32 * dO.abs() @ V.abs().transpose(2, 3) + E_D) + (rel + 4 * f32) * P * (dp.abs() + delta.abs())
+    share = lambda x: x.reshape(B, Hkv, H // Hkv, T, D).sum(2).permute(0, 2, 1, 3)      # noqa: E731
+    E_q = E + (h * ds.abs()).maximum(2.0 ** -33 * ds.abs().amax(-1, keepdim=True))
+    column = ds.abs().reshape(B, Hkv, -1, T).amax(2)[:, :, None].expand(B, Hkv, H // Hkv, T).reshape(B, H, 1, T)
+    E_k = E + (h * ds.abs()).maximum(2.0 ** -33 * column)
+    n = U * (H // Hkv) * f32
+    dq, dk, dv = scale * ds @ K, share(scale * ds.transpose(2, 3) @ Q), share(P.transpose(2, 3) @ dO)
+    return {"out": (back(out), back(E_out)),
+            "dq": (back(dq), rounded(back(dq)) + back(scale * (E_q + T * f32 * ds.abs()) @ K.abs())),
+            "dk": (dk, rounded(dk) + share(scale * (E_k + n * ds.abs()).transpose(2, 3) @ Q.abs())),
+            "dv": (dv, rounded(dv) + share(((h + rel + n) * P + 2.0 ** -39).transpose(2, 3) @ dO.abs()))}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1.0, 300.0])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 8), (2, 40, 1500, 4, 2, 64), (2, 5, 8000, 4, 2, 64), (1, 600, 600, 2, 1, 32), (2, 200, 300, 2, 1, 128), (3, 37, 129, 8, 2, 96),
+                                   (32, 128, 130, 4, 4, 128), (40, 129, 131, 16, 8, 64), (64, 65, 140, 8, 4, 32), (24, 300, 200, 16, 8, 96)], ids=lambda s: "x".join(map(str, s)))
+def test_half_precision_gradients_of_any_size(shape, size):
+    """Output gradients from a mean over many rows (1e-4) to a scaled loss: entries of dS are far below or above what fp16 holds, their sums are not lost."""
+    B, U, T, H, Hkv, D = shape
+    g = torch.Generator().manual_seed(34)
+    r = lambda *s: torch.randn(*s, generator=g)      # noqa: E731
+    q, k, v, dout = ((r(*s) * f + m).half().cuda() for s, f, m in (((B, U, H, D), 1, 0.3), ((B, T, Hkv, D), 1, 0), ((B, T, Hkv, D), 1, 0), ((B, U, H, D), size, 0)))
+    want = half_precision_gradients(q, k, v, dout)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = cross_attention(*leaves)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, dout))):
+        value, bound = want[name]
+        assert torch.isfinite(got).all(), name
+        worst = ((got.double() - value).abs() - bound).max().item()
+        assert worst <= 0, f"{name}: {worst:.3g} over the bound"
+
+
+@pytest.mark.gpu
+def test_half_precision_scores_that_grow_along_the_keys():
+    """The largest dS of a row, and of a key, comes late: what was summed before at a larger scale is carried over."""
+    g = torch.Generator().manual_seed(35)
+    B, U, T, H, Hkv, D = 2, 300, 700, 4, 2, 64
+    r = lambda *s: torch.randn(*s, generator=g)      # noqa: E731
+    q, k = r(B, U, H, D), r(B, T, Hkv, D)
+    q, k = q * torch.logspace(-2, 0, U)[:, None, None], k * torch.logspace(-3, 0.5, T)[:, None, None]
+    v, dout = r(B, T, Hkv, D) * torch.logspace(-3, 1, T)[:, None, None], r(B, U, H, D) * torch.logspace(-4, 1, U)[:, None, None]
+    q, k, v, dout = (x.half().cuda() for x in (q, k, v, dout))
+    want = half_precision_gradients(q, k, v, dout)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(cross_attention(*leaves), leaves, dout)):
+        value, bound = want[name]
+        assert ((got.double() - value).abs() <= bound).all(), name
+
+
+@pytest.mark.gpu
+def test_half_precision_terms_beyond_the_type():
+    """dS above 65504 whose sums, times small keys and queries and the scale, are far below."""
+    g = torch.Generator().manual_seed(36)
+    r = lambda *s: torch.randn(*s, generator=g)      # noqa: E731
+    q, k, v = (x.half().cuda() for x in (0.1 * r(2, 3, 2, 64), 0.01 * r(2, 4, 2, 64), 4 * r(2, 4, 2, 64).sign()))
+    dout = (3e4 * r(2, 3, 2, 64).sign()).half().cuda()
+    want = half_precision_gradients(q, k, v, dout)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(cross_attention(*leaves), leaves, dout)):
+        value, bound = want[name]
+        assert value.abs().max() < 65504 and torch.isfinite(got).all(), name
+        assert ((got.double() - value).abs() <= bound).all(), name
