@@ -209,6 +209,14 @@ def call_on(device, fn, *args):
         check(rc)
 
 
+def refuse_tangents(name, *operands):
+    """Raise where a forward-mode derivative is asked for (``torch.autograd.forward_ad``, ``torch.func.jvp``): a dual tensor does not say
+    ``requires_grad``, and its tangent would be lost without a word."""
+    ad = torch.autograd.forward_ad
+    if ad._current_level >= 0 and any(ad.unpack_dual(t).tangent is not None for t in operands):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def differentiable_once(backward):
     """``torch.autograd.function.once_differentiable`` for a backward that calls the library, without its bookkeeping where no graph of the
     backward is asked for (the ordinary case)."""

@@ -136,7 +136,8 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
     ``query`` (B, U, H, D), ``key`` / ``value`` (B, T, Hkv, D) of one type (fp32, bf16, fp16), any strides; H a multiple of Hkv (query head
     ``h`` reads key head ``h // (H // Hkv)``); D a multiple of 16 bytes, at most 128.  ``key_lengths`` (B,) int32 / int64 on the device: the
     utterances' valid frames (clamped to [0, T]); the frames behind them are never read and get zero gradients, and an utterance without
-    any gives zeros.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once) in query, key and value.
+    any gives zeros.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once,
+    in reverse mode) in query, key and value.
     Scores, softmax and sums are fp32 whatever the type; an infinite value in a valid place gives NaN.  U = 1 is one decode step: the key
     range is split over the GPU where the batch alone does not fill it.  Gradients that nobody asks for are not formed.  Rows that are not
     contiguous or not 16-byte aligned are copied first."""
@@ -144,6 +145,7 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
         scale = float(scale)
         if not 0.0 < scale < math.inf:
             raise RuntimeError(f"cross_attention: scale must be positive, got {scale}")
+    _cabi.refuse_tangents("cross_attention", query, key, value)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _CrossAttentionFn.apply(query, key, value, key_lengths, scale)
     return _forward(query, key, value, key_lengths, scale, False)[6]

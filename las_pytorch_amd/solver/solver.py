@@ -237,7 +237,7 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     among them); ``teacher_index`` (B,U,K) int32 / int64 and ``teacher_logits`` (B,U,K) of any of the three types, K <= 1024: the teacher's
     distribution is the softmax over a row's entries.  Entries with an index outside [0, V) are absent (pad shorter rows with -1); a class named twice
     counts with both entries; a row without entries, like an utterance without steps, adds nothing.  ``lengths`` (B,) int32 / int64 on the
-    device, clamped to [0, U]; None: every step counts.  Returns a scalar fp32 tensor, differentiable (once) in ``pred_y``; its gradient has
+    device, clamped to [0, U]; None: every step counts.  Returns a scalar fp32 tensor, differentiable (once, in reverse mode) in ``pred_y``; its gradient has
     the type of ``pred_y`` and is zero on steps that do not count."""
     if not pred_y.is_cuda:
         raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
@@ -269,6 +269,7 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     if pred_y.stride(2) != 1:
         pred_y = pred_y.contiguous()
     teacher_index, teacher_logits = teacher_index.contiguous(), teacher_logits.contiguous()
+    _cabi.refuse_tangents("distillation_loss_device", pred_y, teacher_logits)
     if torch.is_grad_enabled() and pred_y.requires_grad:
         return _DistillationLoss.apply(pred_y, teacher_index, teacher_logits, lengths, temperature)
     return _distill(pred_y, teacher_index, teacher_logits, lengths, temperature, None)[0]

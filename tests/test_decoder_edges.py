@@ -107,6 +107,44 @@ def test_distillation_backward_addresses_the_tensors_that_arrive(monkeypatch, la
             assert torch.equal(_held_at(at, like, torch.empty(like.shape).stride(), alive), like)
 
 
+def _with_tangents(*operands):
+    """One operand after the other as a dual tensor."""
+    for i, x in enumerate(operands):
+        yield [*operands[:i], torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), *operands[i + 1:]]
+
+
+def test_forward_mode_is_refused_before_the_call(monkeypatch):
+    recorder = Recorder(monkeypatch)
+    operands = _views(torch.float32, "cpu")["plain"]
+    with torch.autograd.forward_ad.dual_level():
+        for duals in _with_tangents(*operands):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cross_attention(*duals)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                cross_attention(*duals)
+        assert not recorder.calls
+        cross_attention(*operands)                      # (no tangent: nothing to lose)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda q: cross_attention(q, *operands[1:]), (operands[0],), (torch.ones_like(operands[0]),))
+    assert len(recorder.calls) == 1
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    operands = _views(torch.float32, "cuda")["plain"]
+    z, index, teacher = torch.randn(2, 3, 9, device="cuda"), torch.zeros(2, 3, 1, dtype=torch.int64, device="cuda"), torch.randn(2, 3, 1, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        for duals in _with_tangents(*operands):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cross_attention(*duals)
+        for z_, teacher_ in _with_tangents(z, teacher):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                S.distillation_loss_device(z_, index, teacher_)
+        assert torch.equal(cross_attention(*operands), cross_attention(*operands))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: S.distillation_loss_device(x, index, teacher), (z,), (torch.ones_like(z),))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("pinned", [False, True], ids=["plain", "pinned"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
