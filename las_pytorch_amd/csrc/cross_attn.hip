@@ -983,7 +983,10 @@ template <class T> int by_dim(const CrossAttnArgs& a, bool bwd, hipStream_t stre
 }  // namespace
 
 // Key ranges of a forward call: as many as fill the chip twice over where the rows alone do not, none shorter than 256 keys (512 at 128 rows, 128 of
-// fp32, whose tiles take longer): a range costs its workgroups a partial result in fp32 and the joining launch.
+// fp32, whose tiles take longer): a range costs its workgroups a partial result in fp32 and the joining launch.  Below 128 rows they are counted in tiles of
+// 32 although fp32 and heads above 64 launch 64 rows: 33 to 64 rows to a key head count as two and are cut only where the GPU is less than half full.  Counted
+// as the one workgroup that they are, heads of 128 over 900 keys: 32 x 4 x 64 rows 23.7 -> 24.4 us bf16, 71 -> 61 fp32; 40 x 4 x 64 23.4 -> 25.7, 72 -> 68; 24 x 4 x 100
+// 22.9 -> 25.1, 71 -> 87; 48 x 4 x 64 over 600 18.1 -> 23.3, 52 -> 66.
 int cross_attn_splits(int B, int U, int T, int H, int Hkv, int dtype) {
     const long R = (long)U * (H / Hkv), per = fwd_wide(B, U, T, H, Hkv) ? 128 : 32, wgs = (long)B * Hkv * ((R + per - 1) / per);
     const long want = wgs >= CA_CUS ? 1 : 2 * CA_CUS / (wgs > 0 ? wgs : 1), most = T / (dtype == 0 ? 128 : per == 128 ? 512 : 256);
