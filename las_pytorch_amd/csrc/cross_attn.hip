@@ -308,7 +308,8 @@ static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
 // the XCDs take turns in that order, so that the last round fills up with the short ones (16 x 512 over ragged 1500: 259 -> 240 us a step).  A
 // permutation of the work for any placement of blocks.
 // TILED: the `per` workgroups lie along the keys, TILED keys each.  Those behind an utterance's end have only zeros to write and start after all others:
-// the shader engines of an XCD take its workgroups in turn, so that one that is done at once leaves its place empty until the turn comes round.
+// the shader engines of an XCD take its workgroups in turn, so that one that is done at once leaves its place empty until the turn comes round.  (Not with
+// ranges of the rows: these are for no more key workgroups than CUs, which all start at once.)
 struct Work { int i, b, kvh; bool any; };      // i: which of the `per` workgroups of (b, kvh)
 template <int TILED = 0> static __device__ __forceinline__ Work work_of(const CrossAttnArgs& a, int block, int per) {
     const int local = block >> 3, n = a.B * a.Hkv, xcd = block & 7;
@@ -324,7 +325,7 @@ template <int TILED = 0> static __device__ __forceinline__ Work work_of(const Cr
     }
     const int sorted = __builtin_amdgcn_ds_permute((lane < a.B ? rank : lane) * 4, lane);
     const int groups = (n + 7) / 8;
-    if (TILED > 0 && groups <= 64) {
+    if (TILED > 0 && a.nk == 1 && groups <= 64) {
         // lane g: the XCD's g-th (utterance, key head), its tiles of keys and of zeros, and their sums up to here
         const bool mine_any = lane < groups && lane * 8 + xcd < n;
         const int b = __shfl(sorted, mine_any ? (lane * 8 + xcd) / a.Hkv : 0), len = __shfl(mine, b);

@@ -8,6 +8,7 @@ import torch
 from las_pytorch_amd import _cabi, cross_attention
 from las_pytorch_amd.model import cross_attention as ca
 from las_pytorch_amd.solver import solver as S
+from test_cross_attention import _check, _inputs
 
 
 class Recorder:
@@ -248,3 +249,12 @@ def test_half_precision_terms_beyond_the_type():
         value, bound = want[name]
         assert value.abs().max() < 65504 and torch.isfinite(got).all(), name
         assert ((got.double() - value).abs() <= bound).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(16, 1000, 100, 8, 1, 64), (8, 2100, 200, 8, 1, 32), (5, 4100, 300, 4, 1, 64)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_ranges_of_rows_of_ragged_utterances(dtype, shape):
+    """Many rows on few keys of different lengths: ranges of the rows and utterances by length in one launch."""
+    q, k, v, dout, lengths = _inputs(dtype, *shape, seed=37)
+    _check(q, k, v, dout, lengths)
