@@ -78,11 +78,12 @@ struct Weigher {
         return y < (float)(SM_BINS - 1) ? (int)y : SM_BINS - 1;
     }
 };
-// x lies in one of the bins up to `bin` (the same comparison that Weigher::bin makes)
+// x can lie in one of the bins up to `bin`: false only where it does not (one comparison; who finds something asks Weigher::bin).  All can where that is the
+// last bin, which also takes the distances that fp32 does not hold: nothing is at least NaN.
 struct Near {
     float zmax, af, most;
-    __device__ __forceinline__ Near(const Weigher& w, int bin) : zmax(w.zmax), af(w.af), most(bin < SM_BINS - 1 ? (float)(bin + 1) : INFINITY) {}
-    __device__ __forceinline__ bool operator()(float x) const { return x == zmax || (zmax - x) * af < most; }
+    __device__ __forceinline__ Near(const Weigher& w, int bin) : zmax(w.zmax), af(w.af), most(bin < SM_BINS - 1 ? (float)(bin + 1) : NAN) {}
+    __device__ __forceinline__ bool operator()(float x) const { return !((zmax - x) * af >= most); }
 };
 static_assert(SM_TABLE == 256, "Weigher::fixed takes the low eight bits");
 

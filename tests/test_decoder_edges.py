@@ -9,6 +9,7 @@ from las_pytorch_amd import _cabi, cross_attention
 from las_pytorch_amd.model import cross_attention as ca
 from las_pytorch_amd.solver import solver as S
 from test_cross_attention import _check, _inputs
+from test_sampling import _check as _check_draws
 
 
 class Recorder:
@@ -258,3 +259,32 @@ def test_ranges_of_rows_of_ragged_utterances(dtype, shape):
     """Many rows on few keys of different lengths: ranges of the rows and utterances by length in one launch."""
     q, k, v, dout, lengths = _inputs(dtype, *shape, seed=37)
     _check(q, k, v, dout, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limits", [dict(top_k=3), dict(top_k=4), dict(top_k=300), dict(top_p=0.9999), dict(top_p=0.5), dict()], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("V", [5, 300, 5000, 20000])
+def test_draws_at_distances_beyond_fp32(V, dtype, limits):
+    """Logits of both ends of the type at a temperature of its size: 6e38 apart, which fp32 does not hold, and 2^-8.7 of the weight all the same."""
+    g = torch.Generator().manual_seed(38)
+    z = torch.full((4, V), -math.inf)
+    for b in range(4):
+        at = torch.randperm(V, generator=g)[:min(V, 400)]
+        z[b, at] = (-1.0 + 0.1 * torch.rand(len(at), generator=g)) * 3e38
+        z[b, at[0]] = 3e38
+    _check_draws(z.to(dtype).cuda(), torch.rand(4, generator=g).cuda(), temperature=1e38, **limits)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [False, True], ids=["one limit", "by row"])
+@pytest.mark.parametrize("V", [300, 5000, 20000])
+def test_few_candidates_at_distances_beyond_fp32(V, rows):
+    """Fewer candidates than top_k may take and all but one of them out of fp32's reach: each random number draws its own."""
+    z = torch.full((8, V), -math.inf)
+    z[:, 7], z[:, 70], z[:, 200] = 3e38, -3e38, -2.9e38
+    # shares of the mass: 1, 2^-8.66 and 2^-8.51 by index
+    u = torch.tensor([0.0, 0.5, 0.99, 0.9945, 0.996, 0.9972, 0.9985, 0.9999], device="cuda")
+    top_k = torch.full((8,), 3, device="cuda") if rows else 3
+    tokens, _ = _check_draws(z.cuda(), u, temperature=1e38, top_k=top_k)
+    assert set(tokens.tolist()) == {7, 70, 200}
