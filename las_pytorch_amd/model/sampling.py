@@ -14,11 +14,11 @@ def _limit(name, value, B, device, whole=False):
     """(scalar, address of a value per row or None, the tensor that must stay alive)."""
     if not torch.is_tensor(value):
         return (int(value) if whole else float(value)), None, None
-    if value.shape != (B,) or value.device != device or value.is_floating_point() == whole or value.dtype == torch.bool:
+    if value.shape != (B,) or value.device != device or value.is_floating_point() == whole or value.is_complex() or value.dtype == torch.bool:
         raise RuntimeError(f"sample_tokens: {name} must be a number or a ({B},) tensor of {'integers' if whole else 'floating numbers'} on the device of the "
                            f"logits, got {tuple(value.shape)} {value.dtype} on {value.device}")
     if whole and value.dtype != torch.int32:
-        value = value.clamp(0, 2 ** 31 - 1).to(torch.int32)
+        value = value.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)      # (narrower types do not hold the bound)
     value = (value if whole else value.to(torch.float32)).contiguous()
     return 0, value.data_ptr(), value
 

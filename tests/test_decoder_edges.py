@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
-from las_pytorch_amd import _cabi, cross_attention
+from las_pytorch_amd import _cabi, cross_attention, sample_tokens
 from las_pytorch_amd.model import cross_attention as ca
+from las_pytorch_amd.model.sampling import _limit
 from las_pytorch_amd.solver import solver as S
 from test_cross_attention import _check, _inputs
 from test_sampling import _check as _check_draws
@@ -288,3 +289,31 @@ def test_few_candidates_at_distances_beyond_fp32(V, rows):
     top_k = torch.full((8,), 3, device="cuda") if rows else 3
     tokens, _ = _check_draws(z.cuda(), u, temperature=1e38, top_k=top_k)
     assert set(tokens.tolist()) == {7, 70, 200}
+
+
+def test_limits_by_row_of_every_type():
+    """What a limit's tensor becomes on its way to the library: int32 or fp32, whatever type it has; other types are refused."""
+    cpu = torch.device("cpu")
+    for dtype in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+        scalar, address, held = _limit("top_k", torch.tensor([0, 3, 100], dtype=dtype), 3, cpu, whole=True)
+        assert scalar == 0 and held.dtype == torch.int32 and held.tolist() == [0, 3, 100] and address == held.data_ptr()
+    assert _limit("top_k", torch.tensor([2 ** 40, -2 ** 40, 7]), 3, cpu, whole=True)[2].tolist() == [2 ** 31 - 1, 0, 7]
+    assert _limit("top_k", torch.tensor([-128, -1, 7], dtype=torch.int8), 3, cpu, whole=True)[2].tolist() == [0, 0, 7]
+    for dtype in (torch.float16, torch.bfloat16, torch.float32, torch.float64):
+        assert _limit("top_p", torch.tensor([0.0, 0.5, 1.0], dtype=dtype), 3, cpu)[2].tolist() == [0.0, 0.5, 1.0]
+    for dtype in (torch.bool, torch.complex64, torch.float32):
+        with pytest.raises(RuntimeError, match="top_k must be"):
+            _limit("top_k", torch.ones(3).to(dtype), 3, cpu, whole=True)
+    for dtype in (torch.bool, torch.complex64, torch.int64):
+        with pytest.raises(RuntimeError, match="top_p must be"):
+            _limit("top_p", torch.ones(3).to(dtype), 3, cpu)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16], ids=lambda t: str(t)[6:])
+def test_top_k_by_row_of_narrow_types(dtype):
+    g = torch.Generator().manual_seed(39)
+    z, u = torch.randn(5, 900, generator=g).cuda() * 2, torch.rand(5, generator=g).cuda()
+    top_k = torch.tensor([0, 1, 2, 50, 127], device="cuda")
+    for a, b in zip(sample_tokens(z, u, top_k=top_k.to(dtype)), sample_tokens(z, u, top_k=top_k)):
+        assert torch.equal(a, b)
