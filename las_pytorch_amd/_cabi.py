@@ -22,6 +22,8 @@ FLAG_GEMM_F32 = 8           # this call's GEMMs on the fp32 matrix pipe (per cal
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # the `dtype` argument of the entry points that take several types
 
+SIZES_BELOW = 1 << 30      # what the entry points of the decoder operators take; ctypes would cut a larger number down to 32 bits without a word
+
 _f = C.c_void_p   # every device pointer is passed as an integer address
 
 

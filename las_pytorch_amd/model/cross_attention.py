@@ -8,7 +8,7 @@ import math
 import torch
 
 from .. import _cabi
-from .._cabi import DTYPES, CrossAttentionDesc, lib
+from .._cabi import DTYPES, SIZES_BELOW, CrossAttentionDesc, lib
 
 
 def _aligned(t):
@@ -30,6 +30,8 @@ def _refuse(query, key, value):
     if key.shape != value.shape or key.shape[0] != B or key.shape[3] != D:
         raise RuntimeError(f"cross_attention: query {tuple(query.shape)}, key {tuple(key.shape)}, value {tuple(value.shape)} do not go together")
     Hkv = key.shape[2]
+    if max(B, _U, key.shape[1], H) >= SIZES_BELOW:
+        raise RuntimeError(f"cross_attention: sizes below 2^30 are needed, got query {tuple(query.shape)}, key {tuple(key.shape)}")
     if H < 1 or Hkv < 1 or H % Hkv:
         raise RuntimeError(f"cross_attention: {H} query heads do not share {Hkv} key heads evenly")
     raise RuntimeError(f"cross_attention: the head size must be a multiple of {4 if query.dtype == torch.float32 else 8} and at most 128, got {D}")
@@ -55,7 +57,7 @@ def _plan(qs, ks, vs, q_strides, k_strides, v_strides, dtype, scale):
     B, U, H, D = qs
     T, Hkv = ks[1], ks[2]
     per16 = 4 if code == 0 else 8
-    if ks[0] != B or ks[3] != D or Hkv < 1 or H < 1 or H % Hkv or not 0 < D <= 128 or D % per16:
+    if max(B, U, T, H) >= SIZES_BELOW or ks[0] != B or ks[3] != D or Hkv < 1 or H < 1 or H % Hkv or not 0 < D <= 128 or D % per16:
         return None
     copied, strides = [], []
     for shape, (sb, st, sh, sd) in ((qs, q_strides), (ks, k_strides), (ks, v_strides)):

@@ -7,7 +7,7 @@ import functools
 import torch
 
 from .. import _cabi
-from .._cabi import DTYPES, lib
+from .._cabi import DTYPES, SIZES_BELOW, lib
 
 
 def _limit(name, value, B, device, whole=False):
@@ -43,6 +43,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in DTYPES:
         raise RuntimeError(f"sample_tokens: logits must be (B,V) in fp32, bf16 or fp16, got {tuple(logits.shape)} {logits.dtype}")
     B, V = logits.shape
+    if max(B, V) >= SIZES_BELOW:
+        raise RuntimeError(f"sample_tokens: sizes below 2^30 are needed, got {tuple(logits.shape)}")
     dev = logits.device
     if uniforms.shape != (B,) or uniforms.dtype != torch.float32 or uniforms.device != dev:
         raise RuntimeError(f"sample_tokens: uniforms must be ({B},) fp32 on the device of the logits, got {tuple(uniforms.shape)} {uniforms.dtype}")

@@ -244,6 +244,8 @@ def distillation_loss_device(pred_y, teacher_index, teacher_logits, temperature=
     if pred_y.dim() != 3 or pred_y.dtype not in _cabi.DTYPES:
         raise RuntimeError(f"distillation_loss_device: pred_y must be (B,U,V) in fp32, bf16 or fp16, got {tuple(pred_y.shape)} {pred_y.dtype}")
     B, U, V = pred_y.shape
+    if max(B, U, V) >= _cabi.SIZES_BELOW:
+        raise RuntimeError(f"distillation_loss_device: sizes below 2^30 are needed, got {tuple(pred_y.shape)}")
     if teacher_index.dim() != 3 or teacher_index.shape[:2] != (B, U) or teacher_index.shape != teacher_logits.shape:
         raise RuntimeError(f"distillation_loss_device: teacher_index {tuple(teacher_index.shape)} and teacher_logits {tuple(teacher_logits.shape)} must "
                            f"both be ({B},{U},K)")

@@ -317,3 +317,29 @@ def test_top_k_by_row_of_narrow_types(dtype):
     top_k = torch.tensor([0, 1, 2, 50, 127], device="cuda")
     for a, b in zip(sample_tokens(z, u, top_k=top_k.to(dtype)), sample_tokens(z, u, top_k=top_k)):
         assert torch.equal(a, b)
+
+
+def test_sizes_that_the_library_would_take_for_smaller_ones():
+    """2^32 + 5 would arrive as 5: nothing is planned for it (stride 0: such a tensor costs no memory)."""
+    x = torch.zeros(1, 1, 1, 8)
+    plan = lambda q, k: ca._plan(q.shape, k.shape, k.shape, q.stride(), k.stride(), k.stride(), q.dtype, None)      # noqa: E731
+    assert plan(x, x.expand(1, 5, 1, 8)) is not None
+    for n in (2 ** 32 + 5, 2 ** 31, 2 ** 30):
+        assert plan(x, x.expand(1, n, 1, 8)) is None and plan(x.expand(1, n, 1, 8), x) is None
+        assert plan(x.expand(n, 1, 1, 8), x.expand(n, 1, 1, 8)) is None and plan(x.expand(1, 1, n, 8), x) is None
+
+
+@pytest.mark.gpu
+def test_sizes_beyond_32_bits_are_refused():
+    x, z = torch.zeros(1, 1, 1, 8, device="cuda"), torch.zeros(1, 1, device="cuda")
+    index = torch.zeros(1, 1, 1, dtype=torch.int64, device="cuda")
+    for n in (2 ** 32 + 5, 2 ** 30):
+        for q, k in ((x, x.expand(1, n, 1, 8)), (x.expand(1, n, 1, 8), x), (x.expand(n, 1, 1, 8), x.expand(n, 1, 1, 8)), (x.expand(1, 1, n, 8), x)):
+            with pytest.raises(RuntimeError, match="2\\^30"):
+                cross_attention(q, k, k)
+        for shape in ((1, n), (n, 1)):
+            with pytest.raises(RuntimeError, match="2\\^30"):
+                sample_tokens(z.expand(shape), z[0].expand(shape[0]))
+        for shape in ((n, 1, 1), (1, n, 1), (1, 1, n)):
+            with pytest.raises(RuntimeError, match="2\\^30"):
+                S.distillation_loss_device(z[None].expand(shape), index.expand(*shape[:2], 1), z[None].expand(*shape[:2], 1))
