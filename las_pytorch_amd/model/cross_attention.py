@@ -93,7 +93,7 @@ def _addressed(d, copied, q, k, v):
         q, k, v = (x.contiguous() if c else x for x, c in zip((q, k, v), copied))
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        strides = [0 if n == 1 else s for x in (q, k, v) for n, s in zip(x.shape[:3], x.stride())]      # (a dimension of one may claim any stride)
         d = CrossAttentionDesc(d.B, d.U, d.T, d.H, d.Hkv, d.D, d.dtype, d.scale, *strides)
     return d, q, k, v
 

@@ -110,6 +110,25 @@ def test_distillation_backward_addresses_the_tensors_that_arrive(monkeypatch, la
             assert torch.equal(_held_at(at, like, torch.empty(like.shape).stride(), alive), like)
 
 
+@pytest.mark.parametrize("between", [False, True], ids=["aligned", "between"])
+def test_strides_of_dimensions_of_one(monkeypatch, between):
+    """The stride of a dimension of one says nothing: one utterance out of a buffer whose rows are no whole 16-byte pieces, beside keys that start between them."""
+    recorder = Recorder(monkeypatch)
+    g = torch.Generator().manual_seed(40)
+    q = torch.randn(3, 5 * 4 * 32 + 1, generator=g)[:, :-1].view(3, 5, 4, 32)[:1]
+    k = torch.randn(9 * 2 * 32 + 1, generator=g)[1:] if between else torch.randn(9 * 2 * 32, generator=g)
+    k = k.view(1, 9, 2, 32)
+    assert q.stride(0) % 4 == 1 and (k.data_ptr() % 16 != 0) == between
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, k)]
+    out = cross_attention(*leaves)
+    torch.autograd.grad(out, leaves, torch.ones_like(out))
+    for d, *addresses in recorder.calls:
+        strides = [getattr(d, n) for n in ("q_b", "q_u", "q_h", "k_b", "k_t", "k_h", "v_b", "v_t", "v_h")]
+        assert not any(s % 4 for s in strides), strides          # (what the library refuses)
+        assert (d.q_u, d.q_h, d.k_t, d.k_h, d.v_t, d.v_h) == (128, 32, 64, 32, 64, 32)
+        assert not any(a % 16 for a in addresses[:3])
+
+
 def _with_tangents(*operands):
     """One operand after the other as a dual tensor."""
     for i, x in enumerate(operands):
