@@ -138,7 +138,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
         const int v = index_at(a, row * a.K + k);
         const float t = v >= 0 ? teacher_at(a, row * a.K + k) : -INFINITY;
         sp[k] = t; si[k] = v;
-        mt = fmaxf(mt, t);
+        mt = t == t ? fmaxf(mt, t) : INFINITY;   // (a NaN, which a maximum would pass over, makes the row's probabilities NaN: NaN - inf)
     }
     if constexpr (NV > 0) {
 #pragma unroll

@@ -362,3 +362,34 @@ def test_sizes_beyond_32_bits_are_refused():
         for shape in ((n, 1, 1), (1, n, 1), (1, 1, n)):
             with pytest.raises(RuntimeError, match="2\\^30"):
                 S.distillation_loss_device(z[None].expand(shape), index.expand(*shape[:2], 1), z[None].expand(*shape[:2], 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [30, 700, 70000])
+@pytest.mark.parametrize("K", [1, 5])
+def test_a_teacher_that_is_not_a_number_is_not_silent(V, K):
+    """A row whose entries are all NaN teaches NaN, as the formula says, not nothing; absent entries may hold anything."""
+    g = torch.Generator().manual_seed(41)
+    z, teacher = torch.randn(2, 3, V, generator=g).cuda(), torch.randn(2, 3, K, generator=g).cuda()
+    index = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(6)]).view(2, 3, K).cuda()
+
+    def step(teacher, index):
+        x = z.clone().requires_grad_(True)
+        loss = S.distillation_loss_device(x, index, teacher, 2.0)
+        return loss.item(), torch.autograd.grad(loss, (x,))[0]
+
+    want_loss, want = step(teacher, index)
+    for entries in (slice(None), slice(0, 1)):
+        bad = teacher.clone()
+        bad[1, 2, entries] = math.nan
+        loss, grad = step(bad, index)
+        assert math.isnan(loss)
+        taught = torch.zeros_like(z, dtype=torch.bool)
+        taught[1, 2, index[1, 2]] = True
+        assert torch.equal(grad.isnan(), taught) and torch.equal(grad[~taught], want[~taught])
+    absent, none = index.clone(), teacher.clone()
+    absent[0, 1], none[0, 1] = -1, math.nan
+    kept = teacher.clone()
+    kept[0, 1] = 0.0
+    assert math.isfinite(step(none, absent)[0]) and step(none, absent)[0] == step(kept, absent)[0]
+    assert not step(none, absent)[1][0, 1].any()
