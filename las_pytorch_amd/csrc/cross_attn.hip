@@ -303,6 +303,13 @@ static __device__ __forceinline__ int length_of(const CrossAttnArgs& a, int b) {
     return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
 }
 
+// The factor that makes a row's sum its output, and its statistic, from the sum l of its exponentials: no key at all gives zeros; keys whose scores are all -inf
+// give NaN, as a score of NaN does.
+static __device__ __forceinline__ float inverse(float l, bool any) { return l > 0.f ? 1.f / l : l == 0.f && !any ? 0.f : NAN; }
+static __device__ __forceinline__ float statistic(float l, bool any, float m, float c, float shift) {
+    return l > 0.f ? fmaf(m, c, log2f(l) - shift) : l == 0.f && !any ? -INFINITY : NAN;
+}
+
 // Which work a block does.  Workgroups of one (utterance, key head) read the same keys: they go to one XCD (blockIdx % 8 on this device) and share its L2.
 // Where a launch takes more than one round of the GPU (`a.longest_first`), an XCD's workgroups start in falling order of their utterances' lengths and
 // the XCDs take turns in that order, so that the last round fills up with the short ones (16 x 512 over ragged 1500: 259 -> 240 us a step).  A
@@ -518,7 +525,7 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
         }
         return;
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);        // (no key at all: zeros; a NaN stays one)
+    const float inv = inverse(l, len > 0);
     T* o = (T*)a.o + out_row * a.D;
 #pragma unroll
     for (int i = 0; i < G::NDT; ++i)
@@ -529,7 +536,7 @@ __global__ __launch_bounds__(CA_THREADS, (FWD_PER_CU<T, DP>)) void cross_attn_fw
             const f32x4 y = {acc[i][4 * x] * inv, acc[i][4 * x + 1] * inv, acc[i][4 * x + 2] * inv, acc[i][4 * x + 3] * inv};
             if (d < a.D) *(V4*)(o + d) = __builtin_convertvector(y, V4);
         }
-    if (a.lse && h == 0) a.lse[out_row] = l > 0.f ? fmaf(m, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
+    if (a.lse && h == 0) a.lse[out_row] = statistic(l, len > 0, m, a.c, P_SHIFT_FWD<T>);
 }
 
 // joins the key ranges of a split forward: four values of one row per thread
@@ -552,11 +559,12 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_kernel(CrossAttnAr
         l += f * ml[(s * n + row) * 2 + 1];
         acc += f * *(const f32x4*)(a.part + (s * n + row) * a.D + d);
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const bool any = length_of(a, (int)(row / ((long)a.U * a.H))) > 0;
+    const float inv = inverse(l, any);
     using V4 = __attribute__((ext_vector_type(4))) T;
     acc *= inv;
     *(V4*)((T*)a.o + row * a.D + d) = __builtin_convertvector(acc, V4);
-    if (a.lse && d == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
+    if (a.lse && d == 0) a.lse[row] = statistic(l, any, mj, a.c, P_SHIFT_FWD<T>);
 }
 
 // The same where there are no more rows than CUs: a workgroup per row, its threads side by side over the ranges too (one token of 16 heads over 100000 frames
@@ -592,11 +600,12 @@ __global__ __launch_bounds__(CA_THREADS) void cross_attn_join_row_kernel(CrossAt
     __syncthreads();
     if (y != 0) return;
     for (int i = 1; i < side; ++i) { acc += sum[i * per + x]; l += ls[i * per + x]; }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const bool any = length_of(a, (int)(row / ((long)a.U * a.H))) > 0;
+    const float inv = inverse(l, any);
     using V4 = __attribute__((ext_vector_type(4))) T;
     acc *= inv;
     *(V4*)((T*)a.o + row * a.D + x * 4) = __builtin_convertvector(acc, V4);
-    if (a.lse && x == 0) a.lse[row] = l > 0.f ? fmaf(mj, a.c, log2f(l) - P_SHIFT_FWD<T>) : (l == 0.f ? -INFINITY : l);
+    if (a.lse && x == 0) a.lse[row] = statistic(l, any, mj, a.c, P_SHIFT_FWD<T>);
 }
 
 // four results of a type, or of fp32 where they are one range's

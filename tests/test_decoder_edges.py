@@ -393,3 +393,31 @@ def test_a_teacher_that_is_not_a_number_is_not_silent(V, K):
     kept[0, 1] = 0.0
     assert math.isfinite(step(none, absent)[0]) and step(none, absent)[0] == step(kept, absent)[0]
     assert not step(none, absent)[1][0, 1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("U, T", [(1, 6), (1, 1500), (40, 70), (150, 1500)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_keys_whose_scores_are_all_minus_infinity(dtype, U, T):
+    """0 / 0: NaN in the output and in the gradients of that utterance; zeros remain those of an utterance without frames; the others keep their bits."""
+    q, k, v, dout, _ = _inputs(dtype, 4, U, T, 4, 2, 64, seed=42)
+    q = q.abs() + 0.5
+    lengths = torch.tensor([T, T // 2, 0, T], dtype=torch.int32, device="cuda")
+
+    def step(k):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = cross_attention(*leaves, lengths)
+        with torch.no_grad():
+            again = cross_attention(*leaves, lengths)
+        assert torch.equal(out.isnan(), again.isnan()) and torch.equal(out[~out.isnan()], again[~again.isnan()])
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    want, bad = step(k), k.clone()
+    bad[1, :T // 2] = -math.inf
+    got = step(bad)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        for i in (0, 2, 3):
+            assert torch.equal(a[i], b[i]), name
+        assert (a[1, :T // 2] if name in ("dk", "dv") else a[1]).isnan().all(), name
+        assert name in ("out", "dq") or not a[1, T // 2:].any(), name
+    assert not got[0][2].any() and not got[1][2].any()
