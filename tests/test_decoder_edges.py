@@ -421,3 +421,31 @@ def test_keys_whose_scores_are_all_minus_infinity(dtype, U, T):
         assert (a[1, :T // 2] if name in ("dk", "dv") else a[1]).isnan().all(), name
         assert name in ("out", "dq") or not a[1, T // 2:].any(), name
     assert not got[0][2].any() and not got[1][2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [30, 3001, 140000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_captured_and_eager_gradients_of_a_scaled_loss_are_one(dtype, V):
+    """A seed other than one goes into the gradient before its rounding, in a graph and outside: the same kernel, the same bits."""
+    g = torch.Generator().manual_seed(43)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()      # noqa: E731
+    z, index, teacher = r(3, 5, V).requires_grad_(True), torch.randint(0, V, (3, 5, 7), generator=g).cuda(), r(3, 5, 7)
+    lengths, seed = torch.tensor([5, 0, 3], dtype=torch.int32, device="cuda"), torch.tensor(3.0, device="cuda")
+
+    def step():
+        loss = S.distillation_loss_device(z, index, teacher, 2.0, lengths)
+        return loss.detach(), *torch.autograd.grad(loss, (z,), seed)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for value in (3.0, 1.0, 1.7e-3, 1024.0):
+        seed.fill_(value)
+        teacher.add_(0.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(step(), held):
+            assert torch.equal(a, b), value
