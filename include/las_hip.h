@@ -276,7 +276,9 @@ int las_sample_tokens(const void* logits, int64_t stride_b, int dtype, int B, in
  *   written there, as zeros).  key_lengths: int32 (B) on the device, values outside [0, T] count as the nearer end; NULL: every frame is valid.
  *   q (B,U,H,D), k / v (B,T,Hkv,D) of one type (dtype 0 fp32, 1 bf16, 2 fp16), any strides (in elements) with rows of D contiguous; row
  *   starts 16-byte aligned; D <= 128, a multiple of 16 bytes.  out / dout / dq (B,U,H,D) and dk / dv (B,T,Hkv,D) contiguous.
- *   lse (B,U,H) fp32: log2 of the sum of exp(s), or -inf; NULL in a forward that no backward follows.  Scores, softmax and sums are fp32.
+ *   lse (B,U,H) fp32: log2 of the sum of exp(s), or -inf; NULL in a forward that no backward follows.  Scores, softmax statistics and sums are fp32; in 16-bit types
+ *   the probabilities and their gradients are rounded to the type for the matrix products that take them (fp16: at a power of two that follows the largest).
+ *   Keys whose scores are all -inf, and NaN, give NaN.
  *   Backward: dq NULL, or dk and dv NULL: that side is not formed (features of a Listener that is not trained).
  *   workspace: las_cross_attention_workspace_floats() floats in the forward, _bwd_workspace_floats() in the backward (0: may be NULL), private to the
  *   call until its kernels have run.
@@ -318,7 +320,9 @@ int las_letter_error_rate(const float* logp, int64_t stride_u, int64_t stride_b,
  *   [0, V) is absent, a class named twice counts with both entries, a row without entries adds nothing.
  *   lengths int32 (B) on the device (clamped to [0, U]) or NULL: all U steps.
  *   loss: 1 float (needs scratch: B U floats), or NULL.  dlogits: gradient of the loss in the logits' type, addressed like them with
- *   dstride_*, or NULL; multiplied by *upstream (device) unless that is NULL.  One pass over the logits either way; no atomics.
+ *   dstride_*, or NULL; multiplied by *upstream (device) unless that is NULL.  The logits are read once up to V = 65536 (fp32) or
+ *   131072 (16-bit), beyond that a second time where the gradient is wanted; no atomics.
+ *   Teacher logits that are all -inf count as none; NaN gives NaN.
  * las_distill_grad_unless_one: the backward of a loss whose forward left its gradient.  dlogits holds it for a factor of one; nothing happens where
  *   *upstream is one, else it is formed anew with the factor inside (rounded to the logits' type once: a scaled loss keeps what fp16 would have lost). */
 typedef struct las_distill_desc {

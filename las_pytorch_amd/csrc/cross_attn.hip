@@ -32,7 +32,7 @@ constexpr int CA_THREADS = 256;
 // Every product runs on the 32x32x16 16-bit matrix instruction (lane half h holds contraction indices 8 h .. 8 h + 7 of 16; accumulation in fp32).
 // A fp32 operand is the exact sum of three bf16 terms (x1 = rne(x), x2 = rne(x - x1), x3 = x - x1 - x2); six of the nine partial products are
 // formed, the other three are below 2^-26 of |a b|: the accuracy of the fp32 matrix instruction at 2.67 times its rate, as in the GEMM.  (An infinite
-// operand becomes NaN on the way: inf - inf.)  The terms of a tile lie in three planes of LDS, split once per workgroup as they are stored.
+// operand becomes NaN on the way, inf - inf, as does one that rounds beyond bf16's largest, 3.39e38.)  The terms of a tile lie in three planes of LDS, split once per workgroup as they are stored.
 template <class T> struct Term { using E = T; static constexpr int N = 1; };
 template <> struct Term<float> { using E = __bf16; static constexpr int N = 3; };
 
@@ -663,6 +663,7 @@ static __device__ __forceinline__ void cross_attn_dq(const CrossAttnArgs& a, int
         qf[c] = dof[c] = no_frag<T>();
         const int d = c * 16 + h * 8;
         if (live) {
+            // (D_i from the output as it was rounded: half a step of each of its values, against a second tensor in fp32 kept from the forward)
             const f32x8 x = values_at((const T*)a.o + out_row * a.D, d, a.D), y = values_at((const T*)a.dout + out_row * a.D, d, a.D);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);

@@ -7,7 +7,8 @@
 // Bound by memory: the logits are read once and their gradient written once, so a row stays in the registers of its workgroup between the
 // statistics and the gradient (up to 16 sixteen-byte pieces per thread of 1024: 131072 16-bit or 65536 fp32 values; longer rows are read
 // a second time).  All statistics are fp32, the sum over rows is formed in a fixed order.  4096 rows of 128000 bf16 classes, 3000 of them taught, with the
-// gradient: 466 us, 4.0 TB/s of bytes read and written.
+// gradient: 466 us, 4.0 TB/s of bytes read and written; behind the registers' end a step
+// of 152000 classes 589 us (of 128000: 483), of 2048 rows of 128000 fp32 classes 541.
 #include "las_common.h"
 #include "las_kernels.h"
 #include <math.h>

@@ -14,8 +14,9 @@
 // One workgroup works at a row where rows alone fill the GPU; otherwise a row is cut into slices (a workgroup each) in four launches: slice
 // maxima, histogram, candidates and slice masses, the draw.  (Letting the row's last workgroup of the third draw at once was measured: its fences
 // write back and drop whole L2s, 139 us at 64 rows of 32000 where that launch now takes a few and the fourth 10.)
-// Bound by latency: 32 rows of 30 logits 10 us a call, 64 rows of 32000 with top-k 15, one row of 128000 with top-p 30 (four launches); and where rows
-// alone fill the GPU by the fp64 weights, 300 cycles of a SIMD each: 241 rows of 31183 with top-p 62 us, without a limit 34.
+// Bound by latency: 32 rows of 30 logits 10 us a call, 64 rows of 32000 with top-k 15, one row of 128000 with top-p 30 (four kernels of 4 + 7 + 10 + 9.5, chains of
+// dependent reads and, in the last, a sort and a scan by one workgroup); and where rows alone fill the GPU by the fp64 weights, 300 cycles of a SIMD each, which
+// top-p has formed twice: 241 rows of 31183 with top-p 60 us, without a limit 33.
 #include "las_common.h"
 #include "las_kernels.h"
 #include <math.h>

@@ -140,7 +140,9 @@ def cross_attention(query, key, value, key_lengths=None, scale=None):
     utterances' valid frames (clamped to [0, T]); the frames behind them are never read and get zero gradients, and an utterance without
     any gives zeros.  ``scale`` (positive) defaults to ``D ** -0.5``.  Returns (B, U, H, D), contiguous; differentiable (once,
     in reverse mode) in query, key and value.
-    Scores, softmax statistics and sums are fp32 whatever the type; what is infinite or NaN in a valid place shows (keys whose scores are all -inf give NaN).  U = 1 is one decode step: the key
+    Scores, softmax statistics and sums are fp32 whatever the type.  In bf16 and fp16 the probabilities and their gradients are rounded to the type for the
+    matrix products that take them (2^-8, 2^-11 of each; in fp16 at a scale that follows the largest), and the backward's inner product of output and its gradient
+    takes the rounded output: about 1.4 times the error of one rounding at the end.  What is infinite or NaN in a valid place shows (keys whose scores are all -inf give NaN).  U = 1 is one decode step: the key
     range is split over the GPU where the batch alone does not fill it.  Gradients that nobody asks for are not formed.  Rows that are not
     contiguous or not 16-byte aligned are copied first."""
     if scale is not None:

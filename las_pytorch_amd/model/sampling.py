@@ -36,8 +36,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     (0: all), of those the ones before which less than ``top_p`` of their mass lies (1: all), of those the ones with ``w >= min_p`` (0:
     all).  The token is the first kept index, in vocabulary order, at which the cumulated mass exceeds ``uniforms`` times the kept
     mass; ``logprob`` is the log of its share.  Each limit is a number or a (B,) tensor on the device (tensors are not read on the host: values
-    outside their range count as off).  ``temperature`` 0 gives the arg-max.  NaN and -inf logits are never drawn; a row of nothing else gives
-    token -1 and logprob -inf.  The same inputs give the same tokens, always."""
+    outside their range count as its nearer end, NaN as off).  ``temperature`` 0 or NaN gives the arg-max.  NaN and -inf logits are never drawn; a row of nothing else gives
+    token -1 and logprob -inf.  The same inputs give the same tokens, always.  No derivative: ``logprob`` is cut off from the graph of ``logits``."""
     if not logits.is_cuda:
         raise RuntimeError("the LAS HIP path needs CUDA(ROCm) tensors; there is no CPU fallback")
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in DTYPES:

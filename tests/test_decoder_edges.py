@@ -449,3 +449,17 @@ def test_captured_and_eager_gradients_of_a_scaled_loss_are_one(dtype, V):
         torch.cuda.synchronize()
         for a, b in zip(step(), held):
             assert torch.equal(a, b), value
+
+
+@pytest.mark.gpu
+def test_a_teacher_of_minus_infinities_teaches_nothing():
+    z, index = torch.randn(2, 3, 50, generator=torch.Generator().manual_seed(44)).cuda(), torch.arange(6, device="cuda").view(2, 3, 1).repeat(1, 1, 4)
+    teacher = torch.randn(2, 3, 4, generator=torch.Generator().manual_seed(45)).cuda()
+    results = []
+    for t, i in ((-math.inf, index[0, 1]), (0.0, -1)):
+        x, told, named = z.clone().requires_grad_(True), teacher.clone(), index.clone()
+        told[0, 1], named[0, 1] = t, i
+        loss = S.distillation_loss_device(x, named, told)
+        results.append((loss.detach(), *torch.autograd.grad(loss, (x,))))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
